@@ -145,8 +145,8 @@ struct Act<bf16_t> {
         return __builtin_bit_cast(uint32_t, h);
     }
     // element-wise a + b, each sum rounded once to bf16 (nearest even).  gfx950 has no packed bf16 add: per pair of
-    // values two unpacks each, ONE packed fp32 add (written on float pairs so that the compiler emits v_pk_add_f32)
-    // and one packed conversion -- 6 instructions instead of 7
+    // values two unpacks each, two fp32 adds (packed fp32 arithmetic is switched off in the build) and one packed
+    // conversion
     static __device__ inline vec8 add8(vec8 a, vec8 b) {
         typedef float f32x2 __attribute__((ext_vector_type(2)));
         typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));

@@ -852,7 +852,7 @@ __global__ __launch_bounds__(NWV * 64) void gemm_tiled_kernel(
         };
         // A wave whose part of the tile lies inside the matrix on both axes (all of them, except along a ragged edge)
         // takes the short way: no bounds checks, so its stores are exactly WN / 2 * WT and the wait behind them can
-        // leave them in flight; scales applied to pairs of values (v_pk_mul_f32), the bias only where there is one;
+        // leave them in flight; scales applied to pairs of values, the bias only where there is one;
         // one store address per wave, the fragments at constant distances from it.
         const bool whole = TL_EPI >= 1 && WN % 2 == 0 && done.t0 + (wt * WT + WT) * 16 <= T &&
                            done.row0 + (wn * WN + WN) * 16 <= done.row_end;
