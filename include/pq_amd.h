@@ -67,6 +67,7 @@ typedef enum pq_status {
 #define PQ_CAP_FUSED_SILU_MUL (1ull << 7) /* pq_gemm_packed_silu_mul runs fused for small batches */
 #define PQ_CAP_EMBEDDING (1ull << 8)      /* pq_embedding */
 #define PQ_CAP_FUSED_ADD_NORM (1ull << 9) /* pq_gemm_packed_add_norm / pq_gemm_packed_normed */
+#define PQ_CAP_FP8_BLOCK (1ull << 10)     /* pq_fp8_* : block-scaled 8-bit floating point linears */
 
 /* Version of this ABI (PQ_ABI_VERSION) and capability bits.  No reference counterpart. */
 int pq_version(void);
@@ -284,6 +285,53 @@ int pq_gemm_packed_normed_silu_mul(const void *xw, int32_t T, int64_t xw_row_str
                                    const void *codebooks, const void *scales, const void *bias /* nullable */, int32_t I,
                                    int32_t G, int32_t K, int32_t d, int32_t code_bytes, int32_t dtype, const float *ssq,
                                    float eps, void *y, int64_t y_row_stride, void *stream);
+
+/*
+ * Linear layers in 8-bit floating point (e4m3: 4 exponent bits, 3 mantissa bits, no infinities, largest value 448), for the
+ * modules of a checkpoint that are not product-quantised.  Weights and activations carry one fp32 scale per block of
+ * PQ_FP8_GROUP = 128 input features: a weight per 128 x 128 block, an activation per token and group.  A last group or
+ * block may be shorter.  fp8 tensors are bytes; "act dtype" is fp16 / bf16 as above.  KB = ceil(K / 128), NB = ceil(N / 128).
+ *   q       [T][K] e4m3, rows q_row_stride bytes apart
+ *   scales  fp32, element (t, b) at t * scale_token_stride + b * scale_group_stride; the quantising entry points write
+ *           scale_token_stride = 1 (tokens adjacent, what the product reads fastest)
+ *   weight  [N][K] e4m3, rows weight_row_stride bytes apart; weight_scales [NB][KB] fp32, rows weight_scales_row_stride apart
+ *
+ * The quantising entry points, for one token's group of values v (fp32, not rounded to the act dtype in between):
+ *   scale = max(max |v|, 2^-96) / 448,  q = e4m3(v / scale), nearest even, the quotient correctly rounded to fp32.
+ * An infinity or NaN in v makes its group's scale infinite / NaN, and with it the token's outputs of a product NaN.
+ *   pq_fp8_group_quant         v = x
+ *   pq_silu_and_mul_fp8        v = silu(x[t][j]) * x[t][I + j], x [T][2 I] (in front of a down_proj held in e4m3)
+ *   pq_rms_norm_fp8            v = x * rsqrt(mean(x^2) + eps) * weight   (in front of qkv_proj / gate_up_proj)
+ *   pq_fused_add_rms_norm_fp8  z = x + residual in fp32, residual <- round(z), v = the norm of z; x is not modified
+ * Rows of up to 16384 values for the norms (15360 where a pointer or stride is not 16-byte aligned or H % 8 != 0).
+ *
+ *   pq_fp8_block_gemm    y[t][n] = round( sum_b scales[t][b] * weight_scales[n / 128][b] * sum_{k in b} q[t][k] *
+ *                        weight[n][k]  + bias[n] ), accumulated in fp32, act dtype y
+ *   pq_fp8_block_linear  pq_fp8_group_quant followed by pq_fp8_block_gemm, the same values.  tmp: 16-byte aligned
+ *                        scratch of pq_fp8_block_linear_tmp_bytes(T, N, K) bytes, free again when the call's work on
+ *                        `stream` is done (NULL is fine where that is 0)
+ * 16-byte aligned rows (pointers and strides) take the fast loads, anything else slower ones; every K, N and T is taken.
+ * No reference counterpart as kernels of this library's form.
+ */
+#define PQ_FP8_GROUP 128
+int pq_fp8_group_quant(const void *x, int64_t x_row_stride, int32_t T, int32_t H, int32_t dtype, void *q,
+                       int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream);
+int pq_silu_and_mul_fp8(const void *x, int64_t x_row_stride, int32_t T, int32_t I, int32_t dtype, void *q,
+                        int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream);
+int pq_rms_norm_fp8(const void *x, int64_t x_row_stride, const void *weight, float eps, int32_t T, int32_t H,
+                    int32_t dtype, void *q, int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream);
+int pq_fused_add_rms_norm_fp8(const void *x, int64_t x_row_stride, void *residual, int64_t res_row_stride,
+                              const void *weight, float eps, int32_t T, int32_t H, int32_t dtype, void *q,
+                              int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream);
+int pq_fp8_block_gemm(const void *q, int32_t T, int64_t q_row_stride, const float *scales, int64_t scale_token_stride,
+                      int64_t scale_group_stride, const void *weight, int64_t weight_row_stride,
+                      const float *weight_scales, int64_t weight_scales_row_stride, const void *bias /* nullable */,
+                      int32_t N, int32_t K, int32_t dtype, void *y, int64_t y_row_stride, void *stream);
+size_t pq_fp8_block_linear_tmp_bytes(int32_t T, int32_t N, int32_t K);
+int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const void *weight, int64_t weight_row_stride,
+                        const float *weight_scales, int64_t weight_scales_row_stride, const void *bias /* nullable */,
+                        int32_t N, int32_t K, int32_t dtype, void *y, int64_t y_row_stride, void *tmp, size_t tmp_bytes,
+                        void *stream);
 
 /*
  * Small-message all-reduce (SUM) between the tensor-parallel ranks of one node, one process per GPU, over device

@@ -23,7 +23,8 @@ EXPORTS = ("pq_version", "pq_caps", "pq_last_error", "pq_dequant", "pq_gemm_work
            "pq_ar_destroy", "pq_ar_all_reduce", "pq_ar_status", "pq_gemm_packed_add_norm_supported",
            "pq_gemm_packed_normed_supported", "pq_gemm_packed_add_norm", "pq_gemm_packed_normed",
            "pq_gemm_packed_normed_silu_mul_supported", "pq_gemm_packed_normed_silu_mul", "pq_ar_add_norm_supported",
-           "pq_ar_all_reduce_add_norm", "pq_ar_set_timeout_ms")
+           "pq_ar_all_reduce_add_norm", "pq_ar_set_timeout_ms", "pq_fp8_group_quant", "pq_silu_and_mul_fp8", "pq_rms_norm_fp8",
+           "pq_fused_add_rms_norm_fp8", "pq_fp8_block_gemm", "pq_fp8_block_linear_tmp_bytes", "pq_fp8_block_linear")
 
 _lock = threading.Lock()
 _lib = None
@@ -107,6 +108,17 @@ def load():
         L.pq_gemm_packed_normed_silu_mul.argtypes = [vp, i32, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp,
                                                      ctypes.c_float, vp, i64, vp]
         L.pq_gemm_packed_normed_silu_mul.restype = ctypes.c_int
+        L.pq_fp8_group_quant.argtypes = [vp, i64, i32, i32, i32, vp, i64, vp, i64, vp]
+        L.pq_silu_and_mul_fp8.argtypes = L.pq_fp8_group_quant.argtypes
+        L.pq_rms_norm_fp8.argtypes = [vp, i64, vp, f32, i32, i32, i32, vp, i64, vp, i64, vp]
+        L.pq_fused_add_rms_norm_fp8.argtypes = [vp, i64, vp, i64, vp, f32, i32, i32, i32, vp, i64, vp, i64, vp]
+        L.pq_fp8_block_gemm.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, i64, vp]
+        L.pq_fp8_block_linear_tmp_bytes.argtypes = [i32, i32, i32]
+        L.pq_fp8_block_linear_tmp_bytes.restype = sz
+        L.pq_fp8_block_linear.argtypes = [vp, i32, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, i64, vp, sz, vp]
+        for fn in ("pq_fp8_group_quant", "pq_silu_and_mul_fp8", "pq_rms_norm_fp8", "pq_fused_add_rms_norm_fp8",
+                   "pq_fp8_block_gemm", "pq_fp8_block_linear"):
+            getattr(L, fn).restype = ctypes.c_int
         L.pq_debug_reload_knobs.argtypes = []
         L.pq_debug_reload_knobs.restype = None
         pvp = ctypes.POINTER(vp)

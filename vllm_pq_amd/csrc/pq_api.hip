@@ -150,7 +150,7 @@ int pq_version(void) { return PQ_ABI_VERSION; }
 
 uint64_t pq_caps(void) {
     return PQ_CAP_DEQUANT | PQ_CAP_GEMM | PQ_CAP_MFMA_SMALL_T | PQ_CAP_MFMA_TILED | PQ_CAP_BF16 | PQ_CAP_FP16 |
-           PQ_CAP_ELEMENTWISE | PQ_CAP_FUSED_SILU_MUL | PQ_CAP_EMBEDDING | PQ_CAP_FUSED_ADD_NORM;
+           PQ_CAP_ELEMENTWISE | PQ_CAP_FUSED_SILU_MUL | PQ_CAP_EMBEDDING | PQ_CAP_FUSED_ADD_NORM | PQ_CAP_FP8_BLOCK;
 }
 
 const char *pq_last_error(void) { return g_err; }
@@ -602,6 +602,153 @@ int pq_gemm_packed_normed_silu_mul(const void *xw, int32_t T, int64_t xw_row_str
     if (!pq::packable(a.parts, G, d, K, 1, code_bytes) || !pq::gemm_decode_act_supported(a))
         return fail(PQ_ERR_UNSUPPORTED, "%s: not a problem the decode kernel fuses (see %s_supported())", fn, fn);
     hipError_t e = pq::launch_gemm_decode_act(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+    return PQ_OK;
+}
+
+// ---- linears in 8-bit floating point ------------------------------------------------------------------------------
+static int fill_quant(pq::QuantArgs &a, const char *fn, const void *x, int64_t x_row_stride, int64_t x_row, int32_t T,
+                      int32_t H, int32_t dtype, void *q, int64_t q_row_stride, float *scales, int64_t scale_group_stride) {
+    int rc = check_rows(fn, T, H, dtype);
+    if (rc) return rc;
+    a = pq::QuantArgs{x, x_row_stride, nullptr, 0, nullptr, 0.f, T, H, dtype, q, q_row_stride, scales, scale_group_stride};
+    if (T == 0 || H == 0) return PQ_OK;
+    if (!x || !q || !scales) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
+    if (x_row_stride < x_row || q_row_stride < H)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: row strides %lld / %lld shorter than the rows (%lld / %d)", fn,
+                    (long long)x_row_stride, (long long)q_row_stride, (long long)x_row, H);
+    if (scale_group_stride < T)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: scale_group_stride=%lld < T=%d", fn, (long long)scale_group_stride, T);
+    return PQ_OK;
+}
+
+int pq_fp8_group_quant(const void *x, int64_t x_row_stride, int32_t T, int32_t H, int32_t dtype, void *q,
+                       int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream) {
+    const char *fn = "pq_fp8_group_quant";
+    pq::QuantArgs a;
+    int rc = fill_quant(a, fn, x, x_row_stride, H, T, H, dtype, q, q_row_stride, scales, scale_group_stride);
+    if (rc) return rc;
+    hipError_t e = pq::launch_group_quant(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+    return PQ_OK;
+}
+
+int pq_silu_and_mul_fp8(const void *x, int64_t x_row_stride, int32_t T, int32_t I, int32_t dtype, void *q,
+                        int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream) {
+    const char *fn = "pq_silu_and_mul_fp8";
+    if (I > INT32_MAX / 2) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: I=%d", fn, I);
+    pq::QuantArgs a;
+    int rc = fill_quant(a, fn, x, x_row_stride, 2 * (int64_t)I, T, I, dtype, q, q_row_stride, scales, scale_group_stride);
+    if (rc) return rc;
+    hipError_t e = pq::launch_silu_quant(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+    return PQ_OK;
+}
+
+static int norm_fp8(const char *fn, const void *x, int64_t x_row_stride, void *residual, int64_t res_row_stride,
+                    const void *weight, float eps, int32_t T, int32_t H, int32_t dtype, void *q, int64_t q_row_stride,
+                    float *scales, int64_t scale_group_stride, void *stream) {
+    pq::QuantArgs a;
+    int rc = fill_quant(a, fn, x, x_row_stride, H, T, H, dtype, q, q_row_stride, scales, scale_group_stride);
+    if (rc) return rc;
+    if (T == 0 || H == 0) return PQ_OK;
+    if (!weight) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
+    if (residual && res_row_stride < H)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: a row stride is shorter than the row (%d)", fn, H);
+    a.residual = residual;
+    a.res_stride = res_row_stride;
+    a.weight = weight;
+    a.eps = eps;
+    if (!pq::norm_quant_vectorised(a) && H > pq::RMS_SCALAR_MAX_H)
+        return fail(PQ_ERR_UNSUPPORTED, "%s: rows of %d elements need 16-byte aligned tensors, strides and H %% 8 == 0 "
+                    "(up to 16384 elements); unaligned rows are supported up to %d", fn, H, pq::RMS_SCALAR_MAX_H);
+    hipError_t e = pq::launch_norm_quant(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+    return PQ_OK;
+}
+
+int pq_rms_norm_fp8(const void *x, int64_t x_row_stride, const void *weight, float eps, int32_t T, int32_t H,
+                    int32_t dtype, void *q, int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream) {
+    return norm_fp8("pq_rms_norm_fp8", x, x_row_stride, nullptr, 0, weight, eps, T, H, dtype, q, q_row_stride, scales,
+                    scale_group_stride, stream);
+}
+
+int pq_fused_add_rms_norm_fp8(const void *x, int64_t x_row_stride, void *residual, int64_t res_row_stride,
+                              const void *weight, float eps, int32_t T, int32_t H, int32_t dtype, void *q,
+                              int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream) {
+    if (T > 0 && H > 0 && !residual) return fail(PQ_ERR_INVALID_ARGUMENT, "pq_fused_add_rms_norm_fp8: residual is NULL");
+    return norm_fp8("pq_fused_add_rms_norm_fp8", x, x_row_stride, residual, res_row_stride, weight, eps, T, H, dtype, q,
+                    q_row_stride, scales, scale_group_stride, stream);
+}
+
+// everything of the product but its activations
+static int fill_fp8_gemm(pq::Fp8GemmArgs &a, const char *fn, int32_t T, const void *weight, int64_t weight_row_stride,
+                         const float *weight_scales, int64_t weight_scales_row_stride, const void *bias, int32_t N,
+                         int32_t K, int32_t dtype, void *y, int64_t y_row_stride) {
+    if (T < 0 || N < 0 || K < 0) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: bad shape T=%d N=%d K=%d", fn, T, N, K);
+    if (dtype != PQ_DTYPE_FP16 && dtype != PQ_DTYPE_BF16)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: dtype=%d is neither fp16 (0) nor bf16 (1)", fn, dtype);
+    if (N > INT32_MAX - 1024 || K > INT32_MAX - 1024) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: N=%d K=%d", fn, N, K);
+    a.w = weight; a.w_stride = weight_row_stride; a.ws = weight_scales; a.ws_stride = weight_scales_row_stride;
+    a.bias = bias; a.T = T; a.N = N; a.K = K; a.dtype = dtype; a.y = y; a.y_stride = y_row_stride;
+    if (T == 0 || N == 0) return PQ_OK;
+    if (!y || (K > 0 && (!weight || !weight_scales))) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
+    if (weight_row_stride < K || y_row_stride < N || weight_scales_row_stride < (K + PQ_FP8_GROUP - 1) / PQ_FP8_GROUP)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: a row stride is shorter than the row (weight %lld, weight_scales %lld, y %lld)",
+                    fn, (long long)weight_row_stride, (long long)weight_scales_row_stride, (long long)y_row_stride);
+    return PQ_OK;
+}
+
+int pq_fp8_block_gemm(const void *q, int32_t T, int64_t q_row_stride, const float *scales, int64_t scale_token_stride,
+                      int64_t scale_group_stride, const void *weight, int64_t weight_row_stride,
+                      const float *weight_scales, int64_t weight_scales_row_stride, const void *bias, int32_t N, int32_t K,
+                      int32_t dtype, void *y, int64_t y_row_stride, void *stream) {
+    const char *fn = "pq_fp8_block_gemm";
+    pq::Fp8GemmArgs a;
+    int rc = fill_fp8_gemm(a, fn, T, weight, weight_row_stride, weight_scales, weight_scales_row_stride, bias, N, K, dtype, y,
+                           y_row_stride);
+    if (rc) return rc;
+    if (T == 0 || N == 0) return PQ_OK;
+    if (K > 0 && (!q || !scales)) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
+    if (q_row_stride < K || scale_token_stride < 0 || scale_group_stride < 0)
+        return fail(PQ_ERR_INVALID_ARGUMENT, "%s: q_row_stride=%lld (K=%d), scale strides %lld / %lld", fn,
+                    (long long)q_row_stride, K, (long long)scale_token_stride, (long long)scale_group_stride);
+    a.q = q; a.q_stride = q_row_stride; a.xs = scales; a.xs_token = scale_token_stride; a.xs_group = scale_group_stride;
+    hipError_t e = pq::launch_fp8_gemm(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+    return PQ_OK;
+}
+
+// tmp of pq_fp8_block_linear: q with rows of K rounded up to 16 bytes, then the scales [KB][T]
+static size_t linear_q_bytes(int32_t T, int32_t K) { return (size_t)T * (((size_t)K + 15) / 16 * 16); }
+
+size_t pq_fp8_block_linear_tmp_bytes(int32_t T, int32_t N, int32_t K) {
+    if (T <= 0 || N <= 0 || K <= 0) return 0;
+    return linear_q_bytes(T, K) + (size_t)T * (((size_t)K + PQ_FP8_GROUP - 1) / PQ_FP8_GROUP) * sizeof(float);
+}
+
+int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const void *weight, int64_t weight_row_stride,
+                        const float *weight_scales, int64_t weight_scales_row_stride, const void *bias, int32_t N, int32_t K,
+                        int32_t dtype, void *y, int64_t y_row_stride, void *tmp, size_t tmp_bytes, void *stream) {
+    const char *fn = "pq_fp8_block_linear";
+    pq::Fp8GemmArgs a;
+    int rc = fill_fp8_gemm(a, fn, T, weight, weight_row_stride, weight_scales, weight_scales_row_stride, bias, N, K, dtype, y,
+                           y_row_stride);
+    if (rc) return rc;
+    if (T == 0 || N == 0) return PQ_OK;
+    if (K > 0 && !x) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
+    if (x_row_stride < K) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: x_row_stride=%lld < K=%d", fn, (long long)x_row_stride, K);
+    const size_t need = pq_fp8_block_linear_tmp_bytes(T, N, K);
+    if (tmp_bytes < need || (need && !tmp))
+        return fail(PQ_ERR_WORKSPACE, "%s: tmp of %zu bytes, %zu needed (pq_fp8_block_linear_tmp_bytes)", fn, tmp_bytes, need);
+    if (reinterpret_cast<uintptr_t>(tmp) & 15) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: tmp must be 16-byte aligned", fn);
+    const int64_t q_stride = ((int64_t)K + 15) / 16 * 16;
+    float *scales = K > 0 ? reinterpret_cast<float *>(static_cast<char *>(tmp) + linear_q_bytes(T, K)) : nullptr;
+    pq::QuantArgs qa{x, x_row_stride, nullptr, 0, nullptr, 0.f, T, K, dtype, tmp, q_stride, scales, T};
+    a.q = tmp; a.q_stride = q_stride; a.xs = scales; a.xs_token = 1; a.xs_group = T;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    hipError_t e = pq::launch_group_quant(qa, s);
+    if (e == hipSuccess) e = pq::launch_fp8_gemm(a, s);
     if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
     return PQ_OK;
 }

@@ -200,6 +200,20 @@ __device__ __forceinline__ float rounded_f32(float f) {
     return f;
 }
 
+// sum over the block, the same value in every thread; fixed order (lane tree, then the waves in order)
+template <int THREADS>
+__device__ inline float block_sum(float v, float *s_part) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) s_part[wave] = v;
+    __syncthreads();
+    float tot = 0.f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) tot += s_part[w];
+    return tot;
+}
+
 // Unsigned index of a signed stored code: value mod K with K a power of two (aqlm.py:32-34).
 template <typename CodeT>
 __device__ inline uint32_t code_index(CodeT c, uint32_t kmask) {

@@ -67,20 +67,6 @@ __global__ __launch_bounds__(EW_THREADS) void silu_and_mul_scalar_kernel(const u
     }
 }
 
-// sum over the block, the same value in every thread; fixed order (lane tree, then the waves in order)
-template <int THREADS>
-__device__ inline float block_sum(float v, float *s_part) {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) s_part[wave] = v;
-    __syncthreads();
-    float tot = 0.f;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) tot += s_part[w];
-    return tot;
-}
-
 // One block of THREADS per token row, NV 8-element pieces per thread kept in registers (rows up to
 // NV * THREADS * 8 elements): as many threads as the row has pieces, so that the whole row is requested at once.
 // ADD: x += residual first.

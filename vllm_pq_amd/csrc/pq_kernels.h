@@ -139,4 +139,44 @@ bool rms_norm_vectorised(const ElementwiseArgs &a);
 hipError_t launch_silu_and_mul(const ElementwiseArgs &a, hipStream_t stream);
 hipError_t launch_rms_norm(const ElementwiseArgs &a, hipStream_t stream);
 
+// Activations in 8-bit floating point (e4m3) with a scale per token and group of FP8_GROUP features (pq_fp8_quant.hip).
+// H = features per token (for the SiLU form the input row holds 2 H); scales[b * scale_stride + t].
+constexpr int FP8_GROUP = PQ_FP8_GROUP;
+constexpr float FP8_MAX = 448.f;   // the largest finite e4m3 value
+struct QuantArgs {
+    const void *x;
+    int64_t x_stride;
+    void *residual;
+    int64_t res_stride;
+    const void *weight;
+    float eps;
+    int T, H, dtype;
+    void *q;
+    int64_t q_stride;
+    float *scales;
+    int64_t scale_stride;
+};
+bool norm_quant_vectorised(const QuantArgs &a);   // else rows of up to RMS_SCALAR_MAX_H
+hipError_t launch_group_quant(const QuantArgs &a, hipStream_t stream);
+hipError_t launch_silu_quant(const QuantArgs &a, hipStream_t stream);
+hipError_t launch_norm_quant(const QuantArgs &a, hipStream_t stream);
+
+// Block-scaled e4m3 matrix product (pq_fp8_gemm.hip): q [T][K], w [N][K] (strides in bytes), xs[t * xs_token + b *
+// xs_group], ws[n / 128 * ws_stride + b].
+struct Fp8GemmArgs {
+    const void *q;
+    int64_t q_stride;
+    const float *xs;
+    int64_t xs_token, xs_group;
+    const void *w;
+    int64_t w_stride;
+    const float *ws;
+    int64_t ws_stride;
+    const void *bias;   // nullable
+    int T, N, K, dtype;
+    void *y;
+    int64_t y_stride;
+};
+hipError_t launch_fp8_gemm(const Fp8GemmArgs &a, hipStream_t stream);
+
 }  // namespace pq

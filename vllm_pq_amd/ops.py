@@ -11,7 +11,7 @@ csrc/quantization/aqlm/gemm_kernels.cu:519-542) and in_features is G * d rather 
 
 Tensors must live on a ROCm device; anything else raises.
 """
-from typing import List, Optional
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -740,6 +740,267 @@ def fused_add_rms_norm(input: torch.Tensor, residual: torch.Tensor, weight: torc
     if _via_op(input, residual):
         return torch.ops.pq_amd.fused_add_rms_norm(input, residual, weight, float(epsilon))
     _fused_add_rms_norm_impl(input, residual, weight, epsilon)
+
+
+# ---- linears in 8-bit floating point (e4m3), one scale per block of 128 ------------------------------
+# include/pq_amd.h states the format and the roundings.  `scales` is [..., ceil(features / 128)] fp32; what the quantising
+# operators return has the tokens adjacent in memory (a transposed view), fp8_block_gemm takes any strides.
+FP8_GROUP = 128
+FP8_DTYPE = torch.float8_e4m3fn
+
+
+def _fp8_input(input: torch.Tensor, what: str):
+    """(2-D rows with unit column stride, row stride); copies what cannot be addressed so."""
+    if input.dtype not in _DTYPE:
+        raise ValueError(f"{what}: fp16 / bf16 activations expected, got {input.dtype}")
+    if input.dim() < 1:
+        raise ValueError(f"{what}: at least one dimension expected")
+    H = input.shape[-1]
+    x2 = input if input.dim() == 2 else input.reshape(-1, H) if input.numel() else input.new_empty((input.shape[:-1].numel(), H))
+    if x2.shape[0] > 1:
+        if x2.stride(1) != 1 or x2.stride(0) < H:
+            x2 = x2.contiguous()
+        return x2, x2.stride(0)
+    return (x2 if x2.stride(1) == 1 else x2.contiguous()), H
+
+
+def _fp8_outputs(input: torch.Tensor, T: int, H: int):
+    """(q [..., H], scales [..., groups] over [groups][T] storage)."""
+    groups = (H + FP8_GROUP - 1) // FP8_GROUP
+    q = torch.empty(input.shape[:-1] + (H,), dtype=FP8_DTYPE, device=input.device)
+    s = torch.empty((groups, T), dtype=torch.float32, device=input.device).t()
+    return q, (s if input.dim() == 2 else s.reshape(input.shape[:-1] + (groups,)))
+
+
+def _fp8_quant_impl(fn: str, input: torch.Tensor, halves: int):
+    dev = _check_device(input)
+    x2, xs = _fp8_input(input, fn[3:])
+    T, W = x2.shape
+    H = W // halves
+    if W != H * halves:
+        raise ValueError(f"{fn[3:]}: input {tuple(input.shape)} does not halve")
+    q, s = _fp8_outputs(input, T, H)
+    if T and H:
+        with _on_device(dev):
+            rc = getattr(_lib.load(), fn)(x2.data_ptr(), xs if T > 1 else W, T, H, _DTYPE[input.dtype], q.data_ptr(), H,
+                                          s.data_ptr(), T, _stream_ptr(dev))
+        if rc:
+            _raise(rc)
+    return q, s
+
+
+def _fp8_norm_impl(input: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, epsilon: float):
+    what = "rms_norm_fp8" if residual is None else "fused_add_rms_norm_fp8"
+    dev = _check_device(input, residual, weight)
+    x2, xs = _fp8_input(input, what)
+    T, H = x2.shape
+    if weight.dtype != input.dtype or (residual is not None and residual.dtype != input.dtype):
+        raise ValueError(f"{what}: input, residual and weight must share one of fp16 / bf16")
+    if weight.shape != (H,) or (residual is not None and residual.shape != input.shape):
+        raise ValueError(f"{what}: shapes {tuple(input.shape)}"
+                         f"{'' if residual is None else f' / {tuple(residual.shape)}'}, weight {tuple(weight.shape)}")
+    r2, rs = _rows(residual, f"{what} residual") if residual is not None and T and H else (None, 0)
+    q, s = _fp8_outputs(input, T, H)
+    if T and H:
+        w = weight.contiguous()
+        L = _lib.load()
+        with _on_device(dev):
+            if r2 is None:
+                rc = L.pq_rms_norm_fp8(x2.data_ptr(), xs, w.data_ptr(), float(epsilon), T, H, _DTYPE[input.dtype],
+                                       q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
+            else:
+                rc = L.pq_fused_add_rms_norm_fp8(x2.data_ptr(), xs, r2.data_ptr(), rs, w.data_ptr(), float(epsilon), T, H,
+                                                 _DTYPE[input.dtype], q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
+        if rc:
+            _raise(rc)
+    return q, s
+
+
+def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor],
+                dtype: torch.dtype):
+    """Checks a block-scaled weight against `K` features; returns (weight, weight_scales, bias) the library can address."""
+    if weight.dtype != FP8_DTYPE or weight.dim() != 2 or weight.shape[1] != K:
+        raise ValueError(f"{what}: weight [out_features, {K}] of {FP8_DTYPE} expected, got {tuple(weight.shape)} {weight.dtype}")
+    N = weight.shape[0]
+    blocks = ((N + FP8_GROUP - 1) // FP8_GROUP, (K + FP8_GROUP - 1) // FP8_GROUP)
+    if weight_scales.dtype != torch.float32 or weight_scales.shape != blocks:
+        raise ValueError(f"{what}: weight_scales {blocks} fp32 expected (one per 128 x 128 block), got "
+                         f"{tuple(weight_scales.shape)} {weight_scales.dtype}")
+    if bias is not None:
+        if bias.numel() != N or bias.dtype != dtype:
+            raise ValueError(f"{what}: bias must hold one value of {dtype} per output row")
+        bias = bias.reshape(-1)
+        if N > 1 and bias.stride(0) != 1:
+            bias = bias.contiguous()
+    if K and (weight.stride(1) != 1 or (N > 1 and weight.stride(0) < K)):
+        weight = weight.contiguous()
+    if not weight_scales.is_contiguous():
+        weight_scales = weight_scales.contiguous()
+    return weight, weight_scales, bias
+
+
+def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                   bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+    what = "fp8_block_gemm"
+    dev = _check_device(input, scales, weight, weight_scales, bias)
+    if input.dtype != FP8_DTYPE or input.dim() < 1:
+        raise ValueError(f"{what}: input of {FP8_DTYPE} expected, got {tuple(input.shape)} {input.dtype}")
+    if out_dtype not in _DTYPE:
+        raise ValueError(f"{what}: out_dtype {out_dtype}: fp16 and bf16 are supported")
+    K = input.shape[-1]
+    groups = (K + FP8_GROUP - 1) // FP8_GROUP
+    if scales.dtype != torch.float32 or scales.shape != input.shape[:-1] + (groups,):
+        raise ValueError(f"{what}: scales {tuple(input.shape[:-1]) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
+    weight, weight_scales, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype)
+    N = weight.shape[0]
+    T = input.shape[:-1].numel()
+    out = torch.empty(input.shape[:-1] + (N,), dtype=out_dtype, device=dev)
+    if T and N:
+        q2 = input if input.dim() == 2 else input.reshape(T, K)
+        if K and (q2.stride(1) != 1 or (T > 1 and q2.stride(0) < K)):
+            q2 = q2.contiguous()
+        s2 = scales if scales.dim() == 2 else scales.reshape(T, groups)
+        with _on_device(dev):
+            rc = _lib.load().pq_fp8_block_gemm(
+                q2.data_ptr(), T, q2.stride(0) if T > 1 else K, s2.data_ptr(), s2.stride(0), s2.stride(1),
+                weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(), groups,
+                bias.data_ptr() if bias is not None else None, N, K, _DTYPE[out_dtype], out.data_ptr(), N, _stream_ptr(dev))
+        if rc:
+            _raise(rc)
+    return out
+
+
+def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                     bias: Optional[torch.Tensor]) -> torch.Tensor:
+    what = "fp8_block_linear"
+    dev = _check_device(input, weight, weight_scales, bias)
+    x2, xs = _fp8_input(input, what)
+    T, K = x2.shape
+    weight, weight_scales, bias = _fp8_weight(what, K, weight, weight_scales, bias, input.dtype)
+    N = weight.shape[0]
+    out = torch.empty(input.shape[:-1] + (N,), dtype=input.dtype, device=dev)
+    if T and N:
+        L = _lib.load()
+        nbytes = L.pq_fp8_block_linear_tmp_bytes(T, N, K)
+        tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        with _on_device(dev):
+            rc = L.pq_fp8_block_linear(
+                x2.data_ptr(), T, xs, weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(),
+                weight_scales.shape[1], bias.data_ptr() if bias is not None else None, N, K, _DTYPE[input.dtype],
+                out.data_ptr(), N, tmp.data_ptr() if tmp is not None else None, nbytes, _stream_ptr(dev))
+        if rc:
+            _raise(rc)
+    return out
+
+
+if _HAVE_CUSTOM_OP:
+
+    def _fp8_fake(input: torch.Tensor, H: int):
+        groups = (H + FP8_GROUP - 1) // FP8_GROUP
+        s = input.new_empty((groups, input.shape[:-1].numel()), dtype=torch.float32).t()
+        return (input.new_empty(input.shape[:-1] + (H,), dtype=FP8_DTYPE),
+                s if input.dim() == 2 else s.reshape(input.shape[:-1] + (groups,)))
+
+    @torch.library.custom_op("pq_amd::fp8_group_quant", mutates_args=(), device_types="cuda")
+    def _fp8_group_quant_op(input: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return _fp8_quant_impl("pq_fp8_group_quant", input, 1)
+
+    @_fp8_group_quant_op.register_fake
+    def _fp8_group_quant_fake(input):
+        return _fp8_fake(input, input.shape[-1])
+
+    @torch.library.custom_op("pq_amd::silu_and_mul_fp8", mutates_args=(), device_types="cuda")
+    def _silu_and_mul_fp8_op(input: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return _fp8_quant_impl("pq_silu_and_mul_fp8", input, 2)
+
+    @_silu_and_mul_fp8_op.register_fake
+    def _silu_and_mul_fp8_fake(input):
+        return _fp8_fake(input, input.shape[-1] // 2)
+
+    @torch.library.custom_op("pq_amd::rms_norm_fp8", mutates_args=(), device_types="cuda")
+    def _rms_norm_fp8_op(input: torch.Tensor, weight: torch.Tensor, epsilon: float) -> Tuple[torch.Tensor, torch.Tensor]:
+        return _fp8_norm_impl(input, None, weight, epsilon)
+
+    @_rms_norm_fp8_op.register_fake
+    def _rms_norm_fp8_fake(input, weight, epsilon):
+        return _fp8_fake(input, input.shape[-1])
+
+    @torch.library.custom_op("pq_amd::fused_add_rms_norm_fp8", mutates_args=("residual",), device_types="cuda")
+    def _fused_add_rms_norm_fp8_op(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                                   epsilon: float) -> Tuple[torch.Tensor, torch.Tensor]:
+        return _fp8_norm_impl(input, residual, weight, epsilon)
+
+    @_fused_add_rms_norm_fp8_op.register_fake
+    def _fused_add_rms_norm_fp8_fake(input, residual, weight, epsilon):
+        return _fp8_fake(input, input.shape[-1])
+
+    @torch.library.custom_op("pq_amd::fp8_block_gemm", mutates_args=(), device_types="cuda")
+    def _fp8_block_gemm_op(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                           bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
+        return _fp8_gemm_impl(input, scales, weight, weight_scales, bias, out_dtype)
+
+    @_fp8_block_gemm_op.register_fake
+    def _fp8_block_gemm_fake(input, scales, weight, weight_scales, bias, out_dtype):
+        return input.new_empty(input.shape[:-1] + (weight.shape[0],), dtype=out_dtype)
+
+    @torch.library.custom_op("pq_amd::fp8_block_linear", mutates_args=(), device_types="cuda")
+    def _fp8_block_linear_op(input: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                             bias: Optional[torch.Tensor]) -> torch.Tensor:
+        return _fp8_linear_impl(input, weight, weight_scales, bias)
+
+    @_fp8_block_linear_op.register_fake
+    def _fp8_block_linear_fake(input, weight, weight_scales, bias):
+        return input.new_empty(input.shape[:-1] + (weight.shape[0],))
+
+
+def fp8_group_quant(input: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scales): `input` [..., H] in e4m3 with one scale per token and group of 128 features, amax / 448."""
+    if _via_op(input):
+        return torch.ops.pq_amd.fp8_group_quant(input)
+    return _fp8_quant_impl("pq_fp8_group_quant", input, 1)
+
+
+def silu_and_mul_fp8(input: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp8_group_quant of silu(input[..., :I]) * input[..., I:], the activation in front of a down_proj held in e4m3
+    (fp32 up to the one rounding to e4m3)."""
+    if _via_op(input):
+        return torch.ops.pq_amd.silu_and_mul_fp8(input)
+    return _fp8_quant_impl("pq_silu_and_mul_fp8", input, 2)
+
+
+def rms_norm_fp8(input: torch.Tensor, weight: torch.Tensor, epsilon: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp8_group_quant of the RMS-normalised input times weight (fp32 up to the one rounding to e4m3)."""
+    if _via_op(input, weight):
+        return torch.ops.pq_amd.rms_norm_fp8(input, weight, float(epsilon))
+    return _fp8_norm_impl(input, None, weight, epsilon)
+
+
+def fused_add_rms_norm_fp8(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                           epsilon: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    """residual += input in place; returns fp8_group_quant of RMS-norm(residual) * weight.  Unlike fused_add_rms_norm,
+    `input` keeps its values (the norm leaves as e4m3)."""
+    if _via_op(input, residual):
+        return torch.ops.pq_amd.fused_add_rms_norm_fp8(input, residual, weight, float(epsilon))
+    if residual is None:
+        raise ValueError("fused_add_rms_norm_fp8: residual expected")
+    return _fp8_norm_impl(input, residual, weight, epsilon)
+
+
+def fp8_block_gemm(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                   bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """y = (input * scales) @ (weight * weight_scales)^T (+ bias) in `out_dtype`, accumulated in fp32: `input` [..., K] and
+    `weight` [N, K] e4m3, `scales` [..., ceil(K / 128)] and `weight_scales` [ceil(N / 128), ceil(K / 128)] fp32."""
+    if _via_op(input, weight):
+        return torch.ops.pq_amd.fp8_block_gemm(input, scales, weight, weight_scales, bias, out_dtype)
+    return _fp8_gemm_impl(input, scales, weight, weight_scales, bias, out_dtype)
+
+
+def fp8_block_linear(input: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                     bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fp8_block_gemm(*fp8_group_quant(input), weight, weight_scales, bias, input.dtype): a linear layer's forward."""
+    if _via_op(input, weight):
+        return torch.ops.pq_amd.fp8_block_linear(input, weight, weight_scales, bias)
+    return _fp8_linear_impl(input, weight, weight_scales, bias)
 
 
 def gemm_kernel_name(T: int, N: int, G: int, M: int, K: int, d: int, code_bytes: int, dtype: torch.dtype,
