@@ -306,11 +306,14 @@ int pq_gemm_packed_normed_silu_mul(const void *xw, int32_t T, int64_t xw_row_str
  * Rows of up to 16384 values for the norms (15360 where a pointer or stride is not 16-byte aligned or H % 8 != 0).
  *
  *   pq_fp8_block_gemm    y[t][n] = round( sum_b scales[t][b] * weight_scales[n / 128][b] * sum_{k in b} q[t][k] *
- *                        weight[n][k]  + bias[n] ), accumulated in fp32, act dtype y
+ *                        weight[n][k]  + bias[n] ), accumulated in fp32, act dtype y.  tmp: optional 16-byte aligned
+ *                        scratch, with which a long K is cut into ranges for more blocks (their sums are added in order);
+ *                        pq_fp8_block_gemm_tmp_bytes(T, N, K) says how much is used at most (0: none)
  *   pq_fp8_block_linear  pq_fp8_group_quant followed by pq_fp8_block_gemm, the same values.  tmp: 16-byte aligned
  *                        scratch of pq_fp8_block_linear_tmp_bytes(T, N, K) bytes, free again when the call's work on
  *                        `stream` is done (NULL is fine where that is 0)
- * 16-byte aligned rows (pointers and strides) take the fast loads, anything else slower ones; every K, N and T is taken.
+ * K, weight, q and their row strides that are multiples of 4 (bytes) take the fast kernels, anything else a slower one;
+ * every T, N and K is taken.  A token's sums may run in another order when T changes; the same call gives the same bits.
  * No reference counterpart as kernels of this library's form.
  */
 #define PQ_FP8_GROUP 128
@@ -323,10 +326,12 @@ int pq_rms_norm_fp8(const void *x, int64_t x_row_stride, const void *weight, flo
 int pq_fused_add_rms_norm_fp8(const void *x, int64_t x_row_stride, void *residual, int64_t res_row_stride,
                               const void *weight, float eps, int32_t T, int32_t H, int32_t dtype, void *q,
                               int64_t q_row_stride, float *scales, int64_t scale_group_stride, void *stream);
+size_t pq_fp8_block_gemm_tmp_bytes(int32_t T, int32_t N, int32_t K);
 int pq_fp8_block_gemm(const void *q, int32_t T, int64_t q_row_stride, const float *scales, int64_t scale_token_stride,
                       int64_t scale_group_stride, const void *weight, int64_t weight_row_stride,
                       const float *weight_scales, int64_t weight_scales_row_stride, const void *bias /* nullable */,
-                      int32_t N, int32_t K, int32_t dtype, void *y, int64_t y_row_stride, void *stream);
+                      int32_t N, int32_t K, int32_t dtype, void *y, int64_t y_row_stride, void *tmp /* nullable */,
+                      size_t tmp_bytes, void *stream);
 size_t pq_fp8_block_linear_tmp_bytes(int32_t T, int32_t N, int32_t K);
 int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const void *weight, int64_t weight_row_stride,
                         const float *weight_scales, int64_t weight_scales_row_stride, const void *bias /* nullable */,

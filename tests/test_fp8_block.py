@@ -70,14 +70,14 @@ def expand(w, ws):
     return w.double() * ws.double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
 
 
-def check_gemm(y, q, s, w, ws, bias):
+def check_gemm(y, q, s, w, ws, bias, dev="cpu"):
     K = w.shape[1]
-    x64 = q.cpu().double().reshape(-1, K) * s.cpu().double().reshape(-1, s.shape[-1]).repeat_interleave(128, 1)[:, :K]
-    w64 = expand(w.cpu(), ws.cpu())
+    x64 = q.to(dev).double().reshape(-1, K) * s.to(dev).double().reshape(-1, s.shape[-1]).repeat_interleave(128, 1)[:, :K]
+    w64 = expand(w.to(dev), ws.to(dev))
     want, mag = x64 @ w64.t(), x64.abs() @ w64.abs().t()
     if bias is not None:
-        want, mag = want + bias.cpu().double(), mag + bias.cpu().double().abs()
-    got = y.cpu().double().reshape(want.shape)
+        want, mag = want + bias.to(dev).double(), mag + bias.to(dev).double().abs()
+    got = y.to(dev).double().reshape(want.shape)
     sums = 7 * 2.0 ** -13 + (32 + blocks(K)) * 2.0 ** -22
     tol = HALF[y.dtype] * want.abs() + sums * mag * (1 + HALF[y.dtype]) + SMALLEST[y.dtype]
     assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
@@ -142,7 +142,7 @@ def _gemm_rc(linear=False, **kw):
     tail = (a["w"], a["wst"], a["ws"], a["wss"], a["b"], a["N"], a["K"], a["dtype"], a["y"], a["ys"])
     if linear:
         return L.pq_fp8_block_linear(a["q"], a["T"], a["qs"], *tail, a["tmp"], a["tb"], None)
-    return L.pq_fp8_block_gemm(a["q"], a["T"], a["qs"], a["s"], a["st"], a["sg"], *tail, None)
+    return L.pq_fp8_block_gemm(a["q"], a["T"], a["qs"], a["s"], a["st"], a["sg"], *tail, a["tmp"], a["tb"], None)
 
 
 @pytest.mark.parametrize("linear", [False, True])
@@ -158,7 +158,7 @@ def test_gemm_refusals_need_no_gpu(linear):
         assert _gemm_rc(True, T=64, tmp=None) == 3 and _gemm_rc(True, T=64, tmp=264) == 1
         assert _lib.load().pq_fp8_block_linear_tmp_bytes(0, 64, 256) == 0
     else:
-        assert _gemm_rc(st=-1) == 1 and _gemm_rc(s=None) == 1
+        assert _gemm_rc(st=-1) == 1 and _gemm_rc(s=None) == 1 and _gemm_rc(tmp=264) == 1
 
 
 def test_ops_raise_on_cpu_tensors():
@@ -282,7 +282,7 @@ def test_gpu_quant_leaves_what_is_outside_its_rows():
 
 # ---- GPU: products ---------------------------------------------------------------------------------
 GEMMS = [(1, 16, 128), (1, 1, 1), (3, 7, 5), (16, 128, 256), (17, 130, 384), (5, 1000, 1080), (33, 96, 2048), (64, 257, 640),
-         (100, 48, 127), (129, 300, 129), (2, 4096, 4096), (333, 1000, 1080), (70, 40, 3000), (257, 513, 528), (300, 640, 131),
+         (100, 48, 127), (129, 300, 129), (2, 4096, 4096), (333, 1000, 1080), (70, 40, 3000), (257, 513, 528), (300, 640, 131), (90, 70, 20), (40, 100, 16), (33, 65, 12), (50, 60, 148),
          (512, 1024, 512), (700, 700, 1600)]
 
 
@@ -303,6 +303,28 @@ def test_gpu_block_gemm_and_linear(T, N, K, dt):
     z = ops.fp8_block_linear(x.to(DEV), w.to(DEV), ws.to(DEV), bd)
     assert z.dtype == DT[dt]
     check_gemm(z, q, s, w, ws, bias)
+
+
+@gpu
+@pytest.mark.parametrize("T,N,K", [(2500, 6100, 1000), (2560, 6144, 1040), (1000, 4000, 1084), (1024, 4096, 512), (520, 4096, 2000),
+                                   (250, 4096, 1152), (64, 512, 8192), (40, 1000, 14300), (300, 4096, 14336), (17, 257, 4100),
+                                   (4096, 300, 260)])
+def test_gpu_block_gemm_tiles(T, N, K):
+    """Sizes that take each tile shape, whole and ragged, with K in one range and in several (the scratch is the caller's: without
+    it the same call runs in one range)."""
+    gen = torch.Generator().manual_seed(T + N + K)
+    q, s = ops.fp8_group_quant(activations(gen, T, K, torch.bfloat16).to(DEV))
+    w, ws = (t.to(DEV) for t in weight(gen, N, K))
+    bias = torch.randn(N, generator=gen).to(torch.bfloat16).to(DEV)
+    y = ops.fp8_block_gemm(q, s, w, ws, bias)
+    check_gemm(y, q, s, w, ws, bias, DEV)
+    if (T, N, K) in ((64, 512, 8192), (40, 1000, 14300)):
+        assert ops._fp8_tmp_bytes("pq_fp8_block_gemm_tmp_bytes", T, N, K) > 0
+    z = torch.empty_like(y)
+    assert _lib.load().pq_fp8_block_gemm(q.data_ptr(), T, K, s.data_ptr(), 1, T, w.data_ptr(), K, ws.data_ptr(), blocks(K),
+                                         bias.data_ptr(), N, K, 1, z.data_ptr(), N, None, 0,
+                                         torch.cuda.current_stream().cuda_stream) == 0
+    check_gemm(z, q, s, w, ws, bias, DEV)
 
 
 @gpu
@@ -365,7 +387,7 @@ def test_gpu_gemm_leaves_what_is_outside_its_rows(T):
     for cols in (N, N - 3):
         y = torch.full((T + 3, N + 8), 31.0, dtype=torch.float16, device=DEV)
         rc = _lib.load().pq_fp8_block_gemm(q.data_ptr(), T, K, s.data_ptr(), s.stride(0), s.stride(1), wd.data_ptr(), K,
-                                           wsd.data_ptr(), 3, None, cols, K, 0, y.data_ptr(), N + 8,
+                                           wsd.data_ptr(), 3, None, cols, K, 0, y.data_ptr(), N + 8, None, 0,
                                            torch.cuda.current_stream().cuda_stream)
         assert rc == 0
         assert (y[T:] == 31).all() and (y[:, cols:] == 31).all()

@@ -24,7 +24,7 @@ EXPORTS = ("pq_version", "pq_caps", "pq_last_error", "pq_dequant", "pq_gemm_work
            "pq_gemm_packed_normed_supported", "pq_gemm_packed_add_norm", "pq_gemm_packed_normed",
            "pq_gemm_packed_normed_silu_mul_supported", "pq_gemm_packed_normed_silu_mul", "pq_ar_add_norm_supported",
            "pq_ar_all_reduce_add_norm", "pq_ar_set_timeout_ms", "pq_fp8_group_quant", "pq_silu_and_mul_fp8", "pq_rms_norm_fp8",
-           "pq_fused_add_rms_norm_fp8", "pq_fp8_block_gemm", "pq_fp8_block_linear_tmp_bytes", "pq_fp8_block_linear")
+           "pq_fused_add_rms_norm_fp8", "pq_fp8_block_gemm", "pq_fp8_block_gemm_tmp_bytes", "pq_fp8_block_linear_tmp_bytes", "pq_fp8_block_linear")
 
 _lock = threading.Lock()
 _lib = None
@@ -112,9 +112,10 @@ def load():
         L.pq_silu_and_mul_fp8.argtypes = L.pq_fp8_group_quant.argtypes
         L.pq_rms_norm_fp8.argtypes = [vp, i64, vp, f32, i32, i32, i32, vp, i64, vp, i64, vp]
         L.pq_fused_add_rms_norm_fp8.argtypes = [vp, i64, vp, i64, vp, f32, i32, i32, i32, vp, i64, vp, i64, vp]
-        L.pq_fp8_block_gemm.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, i64, vp]
-        L.pq_fp8_block_linear_tmp_bytes.argtypes = [i32, i32, i32]
-        L.pq_fp8_block_linear_tmp_bytes.restype = sz
+        L.pq_fp8_block_gemm.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, i64, vp, sz, vp]
+        for fn in (L.pq_fp8_block_gemm_tmp_bytes, L.pq_fp8_block_linear_tmp_bytes):
+            fn.argtypes = [i32, i32, i32]
+            fn.restype = sz
         L.pq_fp8_block_linear.argtypes = [vp, i32, i64, vp, i64, vp, i64, vp, i32, i32, i32, vp, i64, vp, sz, vp]
         for fn in ("pq_fp8_group_quant", "pq_silu_and_mul_fp8", "pq_rms_norm_fp8", "pq_fused_add_rms_norm_fp8",
                    "pq_fp8_block_gemm", "pq_fp8_block_linear"):

@@ -702,7 +702,7 @@ static int fill_fp8_gemm(pq::Fp8GemmArgs &a, const char *fn, int32_t T, const vo
 int pq_fp8_block_gemm(const void *q, int32_t T, int64_t q_row_stride, const float *scales, int64_t scale_token_stride,
                       int64_t scale_group_stride, const void *weight, int64_t weight_row_stride,
                       const float *weight_scales, int64_t weight_scales_row_stride, const void *bias, int32_t N, int32_t K,
-                      int32_t dtype, void *y, int64_t y_row_stride, void *stream) {
+                      int32_t dtype, void *y, int64_t y_row_stride, void *tmp, size_t tmp_bytes, void *stream) {
     const char *fn = "pq_fp8_block_gemm";
     pq::Fp8GemmArgs a;
     int rc = fill_fp8_gemm(a, fn, T, weight, weight_row_stride, weight_scales, weight_scales_row_stride, bias, N, K, dtype, y,
@@ -713,18 +713,28 @@ int pq_fp8_block_gemm(const void *q, int32_t T, int64_t q_row_stride, const floa
     if (q_row_stride < K || scale_token_stride < 0 || scale_group_stride < 0)
         return fail(PQ_ERR_INVALID_ARGUMENT, "%s: q_row_stride=%lld (K=%d), scale strides %lld / %lld", fn,
                     (long long)q_row_stride, K, (long long)scale_token_stride, (long long)scale_group_stride);
+    if (tmp && reinterpret_cast<uintptr_t>(tmp) & 15) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: tmp must be 16-byte aligned", fn);
     a.q = q; a.q_stride = q_row_stride; a.xs = scales; a.xs_token = scale_token_stride; a.xs_group = scale_group_stride;
+    a.tmp = tmp; a.tmp_bytes = tmp_bytes;
     hipError_t e = pq::launch_fp8_gemm(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
     return PQ_OK;
 }
 
-// tmp of pq_fp8_block_linear: q with rows of K rounded up to 16 bytes, then the scales [KB][T]
+size_t pq_fp8_block_gemm_tmp_bytes(int32_t T, int32_t N, int32_t K) {
+    if (T <= 0 || N <= 0 || K <= 0 || N > INT32_MAX - 1024 || K > INT32_MAX - 1024) return 0;
+    return pq::fp8_gemm_tmp_bytes(T, N, K);
+}
+
+// tmp of pq_fp8_block_linear: q with rows of K rounded up to 16 bytes, the scales [KB][T], the product's scratch
 static size_t linear_q_bytes(int32_t T, int32_t K) { return (size_t)T * (((size_t)K + 15) / 16 * 16); }
+static size_t linear_scale_bytes(int32_t T, int32_t K) {
+    return ((size_t)T * (((size_t)K + PQ_FP8_GROUP - 1) / PQ_FP8_GROUP) * sizeof(float) + 15) / 16 * 16;
+}
 
 size_t pq_fp8_block_linear_tmp_bytes(int32_t T, int32_t N, int32_t K) {
     if (T <= 0 || N <= 0 || K <= 0) return 0;
-    return linear_q_bytes(T, K) + (size_t)T * (((size_t)K + PQ_FP8_GROUP - 1) / PQ_FP8_GROUP) * sizeof(float);
+    return linear_q_bytes(T, K) + linear_scale_bytes(T, K) + pq_fp8_block_gemm_tmp_bytes(T, N, K);
 }
 
 int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const void *weight, int64_t weight_row_stride,
@@ -746,6 +756,9 @@ int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const vo
     float *scales = K > 0 ? reinterpret_cast<float *>(static_cast<char *>(tmp) + linear_q_bytes(T, K)) : nullptr;
     pq::QuantArgs qa{x, x_row_stride, nullptr, 0, nullptr, 0.f, T, K, dtype, tmp, q_stride, scales, T};
     a.q = tmp; a.q_stride = q_stride; a.xs = scales; a.xs_token = 1; a.xs_group = T;
+    const size_t head = linear_q_bytes(T, K) + linear_scale_bytes(T, K);
+    a.tmp = need > head ? static_cast<char *>(tmp) + head : nullptr;
+    a.tmp_bytes = need - (need ? head : 0);
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = pq::launch_group_quant(qa, s);
     if (e == hipSuccess) e = pq::launch_fp8_gemm(a, s);

@@ -10,16 +10,10 @@
 #include <string.h>
 
 #include "pq_common.cuh"
+#include "pq_fp8_mfma.cuh"
 #include "pq_kernels.h"
 
 namespace pq {
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// p = sum over one block of 128, no scales (e4m3 x e4m3)
-__device__ __forceinline__ f32x4 mfma_block(const i32x8 &w, const i32x8 &x) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-}
 
 template <bool ALIGNED>
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) {
@@ -39,9 +33,6 @@ __device__ __forceinline__ u32x4 load16_upto(const uint8_t *p, int valid) {
         for (int j = 0; j < 4; ++j)
             if (4 * w + j < valid) v[w] |= (uint32_t)p[4 * w + j] << (8 * j);
     return v;
-}
-__device__ __forceinline__ i32x8 join(const u32x4 &lo, const u32x4 &hi) {
-    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
 // ---- operands straight from memory into registers -------------------------------------------------------------
@@ -165,9 +156,15 @@ static hipError_t direct_at(const Fp8GemmArgs &a, hipStream_t stream) {
 
 template <typename AT>
 static hipError_t fp8_gemm_at(const Fp8GemmArgs &a, hipStream_t stream) {
+    if (a.T > 16 && fp8_gemm_tiled_supported(a)) return launch_fp8_gemm_tiled(a, stream);
     if (a.T <= 16) return direct_at<AT, 1, 1, 4>(a, stream);
-    if (a.T <= 32) return direct_at<AT, 1, 2, 2>(a, stream);
     return direct_at<AT, 2, 4, 1>(a, stream);
+}
+
+// scratch the launch of this problem uses when it gets it (every layout)
+size_t fp8_gemm_tmp_bytes(int T, int N, int K) {
+    if (T <= 16) return 0;
+    return fp8_gemm_tiled_plan(T, N, K, SIZE_MAX).part_bytes;
 }
 
 hipError_t launch_fp8_gemm(const Fp8GemmArgs &a, hipStream_t stream) {

@@ -176,7 +176,15 @@ struct Fp8GemmArgs {
     int T, N, K, dtype;
     void *y;
     int64_t y_stride;
+    void *tmp = nullptr;   // nullable: scratch of launches that cut K into ranges, 16-byte aligned
+    size_t tmp_bytes = 0;
 };
 hipError_t launch_fp8_gemm(const Fp8GemmArgs &a, hipStream_t stream);
+size_t fp8_gemm_tmp_bytes(int T, int N, int K);
+bool fp8_gemm_tiled_supported(const Fp8GemmArgs &a);
+// What the tiled kernel runs with `tmp_bytes` of scratch: tile shape, ranges that K is cut into, bytes of their sums.
+struct Fp8Plan { int shape, ranges; size_t part_bytes; };
+Fp8Plan fp8_gemm_tiled_plan(int T, int N, int K, size_t tmp_bytes);
+hipError_t launch_fp8_gemm_tiled(const Fp8GemmArgs &a, hipStream_t stream);
 
 }  // namespace pq

@@ -11,6 +11,7 @@ csrc/quantization/aqlm/gemm_kernels.cu:519-542) and in_features is G * d rather 
 
 Tensors must live on a ROCm device; anything else raises.
 """
+import functools
 from typing import List, Optional, Tuple
 
 import torch
@@ -839,6 +840,11 @@ def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Te
     return weight, weight_scales, bias
 
 
+@functools.lru_cache(maxsize=4096)
+def _fp8_tmp_bytes(fn: str, T: int, N: int, K: int) -> int:
+    return int(getattr(_lib.load(), fn)(T, N, K))
+
+
 def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                    bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
     what = "fp8_block_gemm"
@@ -860,11 +866,14 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
         if K and (q2.stride(1) != 1 or (T > 1 and q2.stride(0) < K)):
             q2 = q2.contiguous()
         s2 = scales if scales.dim() == 2 else scales.reshape(T, groups)
+        nbytes = _fp8_tmp_bytes("pq_fp8_block_gemm_tmp_bytes", T, N, K)
+        tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _on_device(dev):
             rc = _lib.load().pq_fp8_block_gemm(
                 q2.data_ptr(), T, q2.stride(0) if T > 1 else K, s2.data_ptr(), s2.stride(0), s2.stride(1),
                 weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(), groups,
-                bias.data_ptr() if bias is not None else None, N, K, _DTYPE[out_dtype], out.data_ptr(), N, _stream_ptr(dev))
+                bias.data_ptr() if bias is not None else None, N, K, _DTYPE[out_dtype], out.data_ptr(), N,
+                tmp.data_ptr() if tmp is not None else None, nbytes, _stream_ptr(dev))
         if rc:
             _raise(rc)
     return out
@@ -881,7 +890,7 @@ def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: t
     out = torch.empty(input.shape[:-1] + (N,), dtype=input.dtype, device=dev)
     if T and N:
         L = _lib.load()
-        nbytes = L.pq_fp8_block_linear_tmp_bytes(T, N, K)
+        nbytes = _fp8_tmp_bytes("pq_fp8_block_linear_tmp_bytes", T, N, K)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _on_device(dev):
             rc = L.pq_fp8_block_linear(
