@@ -153,6 +153,7 @@ def test_gemm_refusals_need_no_gpu(linear):
     assert _gemm_rc(linear, T=0) == 0 and _gemm_rc(linear, N=0, ys=0) == 0
     if linear:
         need = _lib.load().pq_fp8_block_linear_tmp_bytes(64, 64, 256)
+        assert _lib.load().pq_fp8_block_linear_tmp_bytes(1, 64, 256) == 0      # quantised inside
         assert need > 0
         assert _gemm_rc(True, T=64, tb=need - 1) == 3 and "tmp" in _lib.last_error()
         assert _gemm_rc(True, T=64, tmp=None) == 3 and _gemm_rc(True, T=64, tmp=264) == 1
@@ -282,7 +283,8 @@ def test_gpu_quant_leaves_what_is_outside_its_rows():
 
 # ---- GPU: products ---------------------------------------------------------------------------------
 GEMMS = [(1, 16, 128), (1, 1, 1), (3, 7, 5), (16, 128, 256), (17, 130, 384), (5, 1000, 1080), (33, 96, 2048), (64, 257, 640),
-         (100, 48, 127), (129, 300, 129), (2, 4096, 4096), (333, 1000, 1080), (70, 40, 3000), (257, 513, 528), (300, 640, 131), (90, 70, 20), (40, 100, 16), (33, 65, 12), (50, 60, 148),
+         (100, 48, 127), (129, 300, 129), (2, 4096, 4096), (333, 1000, 1080), (70, 40, 3000), (257, 513, 528), (300, 640, 131), (90, 70, 20), (40, 100, 16), (33, 65, 12), (50, 60, 148), (2, 100, 20), (16, 40, 4100), (4, 8200, 144), (9, 64, 8200),
+         (16, 96, 14336), (3, 50, 16384), (4, 33, 16400), (1, 9000, 1024), (7, 33, 131), (16, 20, 257), (1, 40, 1003), (2, 300, 4098), (8, 48, 1024),
          (512, 1024, 512), (700, 700, 1600)]
 
 
@@ -303,6 +305,8 @@ def test_gpu_block_gemm_and_linear(T, N, K, dt):
     z = ops.fp8_block_linear(x.to(DEV), w.to(DEV), ws.to(DEV), bd)
     assert z.dtype == DT[dt]
     check_gemm(z, q, s, w, ws, bias)
+    if K % 4 == 0:      # the quantised rows have the same layout to both: the same kernel, the same bits
+        assert torch.equal(y, z)
 
 
 @gpu

@@ -733,7 +733,7 @@ static size_t linear_scale_bytes(int32_t T, int32_t K) {
 }
 
 size_t pq_fp8_block_linear_tmp_bytes(int32_t T, int32_t N, int32_t K) {
-    if (T <= 0 || N <= 0 || K <= 0) return 0;
+    if (T <= 0 || N <= 0 || K <= 0 || pq::fp8_linear_fused(T, K)) return 0;
     return linear_q_bytes(T, K) + linear_scale_bytes(T, K) + pq_fp8_block_gemm_tmp_bytes(T, N, K);
 }
 
@@ -748,6 +748,15 @@ int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const vo
     if (T == 0 || N == 0) return PQ_OK;
     if (K > 0 && !x) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
     if (x_row_stride < K) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: x_row_stride=%lld < K=%d", fn, (long long)x_row_stride, K);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    a.q = x; a.q_stride = x_row_stride;
+    if (pq::fp8_linear_fused(T, K) && K > 0) {
+        if (weight_row_stride >= (1 << 26))
+            return fail(PQ_ERR_UNSUPPORTED, "%s: weight_row_stride=%lld", fn, (long long)weight_row_stride);
+        hipError_t e = pq::launch_fp8_linear_fused(a, s);
+        if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
+        return PQ_OK;
+    }
     const size_t need = pq_fp8_block_linear_tmp_bytes(T, N, K);
     if (tmp_bytes < need || (need && !tmp))
         return fail(PQ_ERR_WORKSPACE, "%s: tmp of %zu bytes, %zu needed (pq_fp8_block_linear_tmp_bytes)", fn, tmp_bytes, need);
@@ -759,7 +768,6 @@ int pq_fp8_block_linear(const void *x, int32_t T, int64_t x_row_stride, const vo
     const size_t head = linear_q_bytes(T, K) + linear_scale_bytes(T, K);
     a.tmp = need > head ? static_cast<char *>(tmp) + head : nullptr;
     a.tmp_bytes = need - (need ? head : 0);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     hipError_t e = pq::launch_group_quant(qa, s);
     if (e == hipSuccess) e = pq::launch_fp8_gemm(a, s);
     if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));

@@ -144,6 +144,31 @@ __global__ __launch_bounds__(WK * 64) void fp8_gemm_direct_kernel(Fp8GemmArgs a)
     }
 }
 
+// y = round(sum of the K ranges' sums + bias): 4 features of one token per thread, the ranges in order
+template <typename AT>
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float *part, int split, int T, int N, int64_t np, const uint16_t *bias,
+                                                       uint16_t *y, int64_t y_stride) {
+    const int64_t per = np / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= T * per) return;
+    const int64_t t = i / per;
+    const int n = (int)(i - t * per) * 4;
+    f32x4 v = *reinterpret_cast<const f32x4 *>(part + t * np + n);
+    for (int k = 1; k < split; ++k) v += *reinterpret_cast<const f32x4 *>(part + ((int64_t)k * T + t) * np + n);
+    uint16_t *row = y + t * y_stride + n;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < N) row[e] = Act<AT>::from_f32(v[e] + (bias ? Act<AT>::to_f32(bias[n + e]) : 0.f));
+}
+
+hipError_t launch_fp8_join(const Fp8GemmArgs &a, const float *part, int ranges, int64_t np, hipStream_t stream) {
+    const dim3 grid((unsigned)((a.T * (np / 4) + 255) / 256)), block(256);
+    const uint16_t *bias = static_cast<const uint16_t *>(a.bias);
+    uint16_t *y = static_cast<uint16_t *>(a.y);
+    if (a.dtype == PQ_DTYPE_BF16) hipLaunchKernelGGL((fp8_join_kernel<bf16_t>), grid, block, 0, stream, part, ranges, a.T, a.N, np, bias, y, a.y_stride);
+    else hipLaunchKernelGGL((fp8_join_kernel<fp16_t>), grid, block, 0, stream, part, ranges, a.T, a.N, np, bias, y, a.y_stride);
+    return hipGetLastError();
+}
+
 template <typename AT, int NF, int TF, int U>
 static hipError_t direct_at(const Fp8GemmArgs &a, hipStream_t stream) {
     constexpr int WK = 8;
@@ -156,15 +181,15 @@ static hipError_t direct_at(const Fp8GemmArgs &a, hipStream_t stream) {
 
 template <typename AT>
 static hipError_t fp8_gemm_at(const Fp8GemmArgs &a, hipStream_t stream) {
-    if (a.T > 16 && fp8_gemm_tiled_supported(a)) return launch_fp8_gemm_tiled(a, stream);
+    if (fp8_gemm_stream_supported(a)) return launch_fp8_gemm_stream(a, stream);
+    if (fp8_gemm_tiled_supported(a)) return launch_fp8_gemm_tiled(a, stream);
     if (a.T <= 16) return direct_at<AT, 1, 1, 4>(a, stream);
     return direct_at<AT, 2, 4, 1>(a, stream);
 }
 
 // scratch the launch of this problem uses when it gets it (every layout)
 size_t fp8_gemm_tmp_bytes(int T, int N, int K) {
-    if (T <= 16) return 0;
-    return fp8_gemm_tiled_plan(T, N, K, SIZE_MAX).part_bytes;
+    return T <= 16 ? fp8_gemm_stream_tmp_bytes(T, N, K) : fp8_gemm_tiled_plan(T, N, K, SIZE_MAX).part_bytes;
 }
 
 hipError_t launch_fp8_gemm(const Fp8GemmArgs &a, hipStream_t stream) {

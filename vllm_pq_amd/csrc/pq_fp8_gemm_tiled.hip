@@ -323,22 +323,6 @@ __global__ __launch_bounds__(WN * WT * KG * 64) void fp8_gemm_tiled_kernel(Fp8Ge
     }
 }
 
-// y = round(sum of the K ranges' sums + bias): 4 features of one token per thread, the ranges in order
-template <typename AT>
-__global__ __launch_bounds__(256) void fp8_join_kernel(const float *part, int split, int T, int N, int64_t np, const uint16_t *bias,
-                                                       uint16_t *y, int64_t y_stride) {
-    const int64_t per = np / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= T * per) return;
-    const int64_t t = i / per;
-    const int n = (int)(i - t * per) * 4;
-    f32x4 v = *reinterpret_cast<const f32x4 *>(part + t * np + n);
-    for (int k = 1; k < split; ++k) v += *reinterpret_cast<const f32x4 *>(part + ((int64_t)k * T + t) * np + n);
-    uint16_t *row = y + t * y_stride + n;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (n + e < N) row[e] = Act<AT>::from_f32(v[e] + (bias ? Act<AT>::to_f32(bias[n + e]) : 0.f));
-}
-
 template <typename AT, int BN, int BT, int WN, int WT, int KG, int STAGES>
 static hipError_t tiled_at(const Fp8GemmArgs &a, int split, hipStream_t stream) {
     typedef Fp8Tile<BN, BT, WN, WT, KG, STAGES> C;
@@ -361,10 +345,7 @@ static hipError_t tiled_at(const Fp8GemmArgs &a, int split, hipStream_t stream) 
     hipLaunchKernelGGL(kern, dim3((unsigned)(per_xcd * 8), (unsigned)split), dim3(C::THREADS), C::LDS, stream, a, tn, tt, (int)per_xcd,
                        kb_split, part, np);
     e = hipGetLastError();
-    if (e != hipSuccess || !part) return e;
-    hipLaunchKernelGGL((fp8_join_kernel<AT>), dim3((unsigned)((a.T * (np / 4) + 255) / 256)), dim3(256), 0, stream, part, split, a.T,
-                       a.N, np, static_cast<const uint16_t *>(a.bias), static_cast<uint16_t *>(a.y), a.y_stride);
-    return hipGetLastError();
+    return e != hipSuccess || !part ? e : launch_fp8_join(a, part, split, np, stream);
 }
 
 bool fp8_gemm_tiled_supported(const Fp8GemmArgs &a) {

@@ -16,44 +16,14 @@
 #include <hip/hip_runtime.h>
 
 #include "pq_common.cuh"
+#include "pq_fp8_scale.cuh"
 #include "pq_kernels.h"
 
 namespace pq {
 
 constexpr int QT = 256;                  // threads per block of the quantising kernels without a norm
 constexpr int QV = FP8_GROUP / 8;        // threads per group
-constexpr uint32_t AMAX_MIN_BITS = (127 - 96) << 23;   // 2^-96
 
-// What divides a group: s, and what the quotient is corrected with.
-struct GroupScale {
-    float s, r, c;
-};
-__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
-    GroupScale g;
-    g.s = __uint_as_float(amax_bits > AMAX_MIN_BITS ? amax_bits : AMAX_MIN_BITS) / FP8_MAX;
-    g.r = 1.0f / g.s;
-    g.c = __builtin_isinf(g.s) ? 0.f : g.s;   // an infinite scale: v * r stands as it is (0, or NaN for the infinity itself)
-    return g;
-}
-// v / s, correctly rounded: a product with the rounded reciprocal is within two units of the last place, one Newton step
-// on the exact residual brings it within one, and from there a second step rounds as division does (Markstein's theorem).
-// Half the instructions of a division; a plain product would move values that lie on a tie between two e4m3 numbers, which
-// is common with act-dtype inputs.
-__device__ __forceinline__ float div_group(float v, const GroupScale &g) {
-    float q = v * g.r;
-    q = __builtin_fmaf(__builtin_fmaf(-q, g.c, v), g.r, q);
-    return __builtin_fmaf(__builtin_fmaf(-q, g.c, v), g.r, q);
-}
-__device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-// four values -> four e4m3 bytes
-__device__ __forceinline__ uint32_t pack4(const float *v, const GroupScale &g) {
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(div_group(v[0], g), div_group(v[1], g), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(div_group(v[2], g), div_group(v[3], g), p, true);
-}
-__device__ __forceinline__ uint8_t pack1(float v, const GroupScale &g) {
-    return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(div_group(v, g), 0.f, 0, false);
-}
 // maximum over the 16 lanes of a group
 __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 #pragma unroll

@@ -181,6 +181,14 @@ struct Fp8GemmArgs {
 };
 hipError_t launch_fp8_gemm(const Fp8GemmArgs &a, hipStream_t stream);
 size_t fp8_gemm_tmp_bytes(int T, int N, int K);
+// y from the sums [ranges][T][np] of a K cut into ranges, added in order.
+hipError_t launch_fp8_join(const Fp8GemmArgs &a, const float *part, int ranges, int64_t np, hipStream_t stream);
+bool fp8_gemm_stream_supported(const Fp8GemmArgs &a);     // up to 16 tokens
+size_t fp8_gemm_stream_tmp_bytes(int T, int N, int K);
+hipError_t launch_fp8_gemm_stream(const Fp8GemmArgs &a, hipStream_t stream);
+// The same product from fp16 / bf16 activations (a.q, a.q_stride in elements; a.xs unused), quantised inside.
+bool fp8_linear_fused(int T, int K);       // whether a linear of this size takes it (w_stride < 2^26)
+hipError_t launch_fp8_linear_fused(const Fp8GemmArgs &a, hipStream_t stream);
 bool fp8_gemm_tiled_supported(const Fp8GemmArgs &a);
 // What the tiled kernel runs with `tmp_bytes` of scratch: tile shape, ranges that K is cut into, bytes of their sums.
 struct Fp8Plan { int shape, ranges; size_t part_bytes; };

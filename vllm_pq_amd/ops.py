@@ -750,41 +750,57 @@ FP8_GROUP = 128
 FP8_DTYPE = torch.float8_e4m3fn
 
 
-def _fp8_input(input: torch.Tensor, what: str):
-    """(2-D rows with unit column stride, row stride); copies what cannot be addressed so."""
-    if input.dtype not in _DTYPE:
+# These calls are on the host path of launches that run for a few microseconds: the checks take the common case (2-D rows,
+# everything contiguous on the current device) first and allocate each output in one call.
+def _fp8_act(input: torch.Tensor, what: str):
+    """(2-D rows with unit column stride, tokens, features, row stride, device, dtype code); copies what cannot be addressed
+    so."""
+    code = _DTYPE.get(input.dtype)
+    if code is None or not input.is_cuda:
+        _check_device(input)
         raise ValueError(f"{what}: fp16 / bf16 activations expected, got {input.dtype}")
-    if input.dim() < 1:
-        raise ValueError(f"{what}: at least one dimension expected")
-    H = input.shape[-1]
-    x2 = input if input.dim() == 2 else input.reshape(-1, H) if input.numel() else input.new_empty((input.shape[:-1].numel(), H))
-    if x2.shape[0] > 1:
-        if x2.stride(1) != 1 or x2.stride(0) < H:
-            x2 = x2.contiguous()
-        return x2, x2.stride(0)
-    return (x2 if x2.stride(1) == 1 else x2.contiguous()), H
+    if input.dim() != 2:
+        if input.dim() < 1:
+            raise ValueError(f"{what}: at least one dimension expected")
+        T, H = input.shape[:-1].numel(), input.shape[-1]
+        x2 = input.reshape(T, H)
+    else:
+        x2 = input
+        T, H = input.shape
+    s0, s1 = x2.stride()
+    if (s1 != 1 and H > 1) or (s0 < H and T > 1):
+        x2 = x2.contiguous()
+        s0 = H
+    return x2, T, H, (s0 if T > 1 else H), input.device, code
 
 
-def _fp8_outputs(input: torch.Tensor, T: int, H: int):
+def _fp8_outputs(input: torch.Tensor, T: int, H: int, dev):
     """(q [..., H], scales [..., groups] over [groups][T] storage)."""
     groups = (H + FP8_GROUP - 1) // FP8_GROUP
-    q = torch.empty(input.shape[:-1] + (H,), dtype=FP8_DTYPE, device=input.device)
-    s = torch.empty((groups, T), dtype=torch.float32, device=input.device).t()
-    return q, (s if input.dim() == 2 else s.reshape(input.shape[:-1] + (groups,)))
+    s = torch.empty_strided((T, groups), (1, T), dtype=torch.float32, device=dev)
+    if input.dim() == 2:
+        return input.new_empty((T, H), dtype=FP8_DTYPE), s
+    lead = input.shape[:-1]
+    return input.new_empty(lead + (H,), dtype=FP8_DTYPE), s.reshape(lead + (groups,))
+
+
+def _on_current(dev) -> bool:
+    return dev.index == torch.cuda.current_device()
 
 
 def _fp8_quant_impl(fn: str, input: torch.Tensor, halves: int):
-    dev = _check_device(input)
-    x2, xs = _fp8_input(input, fn[3:])
-    T, W = x2.shape
+    x2, T, W, xs, dev, code = _fp8_act(input, fn[3:])
     H = W // halves
     if W != H * halves:
         raise ValueError(f"{fn[3:]}: input {tuple(input.shape)} does not halve")
-    q, s = _fp8_outputs(input, T, H)
+    q, s = _fp8_outputs(input, T, H, dev)
     if T and H:
-        with _on_device(dev):
-            rc = getattr(_lib.load(), fn)(x2.data_ptr(), xs if T > 1 else W, T, H, _DTYPE[input.dtype], q.data_ptr(), H,
-                                          s.data_ptr(), T, _stream_ptr(dev))
+        call = getattr(_lib.load(), fn)
+        if _on_current(dev):
+            rc = call(x2.data_ptr(), xs, T, H, code, q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
+        else:
+            with _on_device(dev):
+                rc = call(x2.data_ptr(), xs, T, H, code, q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
         if rc:
             _raise(rc)
     return q, s
@@ -792,34 +808,38 @@ def _fp8_quant_impl(fn: str, input: torch.Tensor, halves: int):
 
 def _fp8_norm_impl(input: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, epsilon: float):
     what = "rms_norm_fp8" if residual is None else "fused_add_rms_norm_fp8"
-    dev = _check_device(input, residual, weight)
-    x2, xs = _fp8_input(input, what)
-    T, H = x2.shape
+    x2, T, H, xs, dev, code = _fp8_act(input, what)
+    if weight.device != dev or (residual is not None and residual.device != dev):
+        _check_device(input, residual, weight)
     if weight.dtype != input.dtype or (residual is not None and residual.dtype != input.dtype):
         raise ValueError(f"{what}: input, residual and weight must share one of fp16 / bf16")
     if weight.shape != (H,) or (residual is not None and residual.shape != input.shape):
         raise ValueError(f"{what}: shapes {tuple(input.shape)}"
                          f"{'' if residual is None else f' / {tuple(residual.shape)}'}, weight {tuple(weight.shape)}")
     r2, rs = _rows(residual, f"{what} residual") if residual is not None and T and H else (None, 0)
-    q, s = _fp8_outputs(input, T, H)
+    q, s = _fp8_outputs(input, T, H, dev)
     if T and H:
-        w = weight.contiguous()
+        w = weight if weight.is_contiguous() else weight.contiguous()
         L = _lib.load()
         with _on_device(dev):
             if r2 is None:
-                rc = L.pq_rms_norm_fp8(x2.data_ptr(), xs, w.data_ptr(), float(epsilon), T, H, _DTYPE[input.dtype],
-                                       q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
+                rc = L.pq_rms_norm_fp8(x2.data_ptr(), xs, w.data_ptr(), epsilon, T, H, code, q.data_ptr(), H, s.data_ptr(), T,
+                                       _stream_ptr(dev))
             else:
-                rc = L.pq_fused_add_rms_norm_fp8(x2.data_ptr(), xs, r2.data_ptr(), rs, w.data_ptr(), float(epsilon), T, H,
-                                                 _DTYPE[input.dtype], q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
+                rc = L.pq_fused_add_rms_norm_fp8(x2.data_ptr(), xs, r2.data_ptr(), rs, w.data_ptr(), epsilon, T, H, code,
+                                                 q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
         if rc:
             _raise(rc)
     return q, s
 
 
 def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Tensor, bias: Optional[torch.Tensor],
-                dtype: torch.dtype):
-    """Checks a block-scaled weight against `K` features; returns (weight, weight_scales, bias) the library can address."""
+                dtype: torch.dtype, dev):
+    """Checks a block-scaled weight against `K` features; returns (weight, its row stride, N, weight_scales, bias pointer,
+    bias) that the library can address."""
+    if weight.device != dev or weight_scales.device != dev or (bias is not None and bias.device != dev):
+        _check_device(weight, weight_scales, bias)
+        raise RuntimeError(f"{what}: weight on {weight.device}, activations on {dev}")
     if weight.dtype != FP8_DTYPE or weight.dim() != 2 or weight.shape[1] != K:
         raise ValueError(f"{what}: weight [out_features, {K}] of {FP8_DTYPE} expected, got {tuple(weight.shape)} {weight.dtype}")
     N = weight.shape[0]
@@ -830,14 +850,14 @@ def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Te
     if bias is not None:
         if bias.numel() != N or bias.dtype != dtype:
             raise ValueError(f"{what}: bias must hold one value of {dtype} per output row")
-        bias = bias.reshape(-1)
-        if N > 1 and bias.stride(0) != 1:
-            bias = bias.contiguous()
-    if K and (weight.stride(1) != 1 or (N > 1 and weight.stride(0) < K)):
+        bias = bias.reshape(-1).contiguous()
+    w0, w1 = weight.stride()
+    if (w1 != 1 and K > 1) or (w0 < K and N > 1):
         weight = weight.contiguous()
+        w0 = K
     if not weight_scales.is_contiguous():
         weight_scales = weight_scales.contiguous()
-    return weight, weight_scales, bias
+    return weight, (w0 if N > 1 else K), N, weight_scales, (None if bias is None else bias.data_ptr()), bias
 
 
 @functools.lru_cache(maxsize=4096)
@@ -848,32 +868,35 @@ def _fp8_tmp_bytes(fn: str, T: int, N: int, K: int) -> int:
 def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                    bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
     what = "fp8_block_gemm"
-    dev = _check_device(input, scales, weight, weight_scales, bias)
+    if not input.is_cuda or scales.device != input.device:
+        _check_device(input, scales, weight, weight_scales, bias)
     if input.dtype != FP8_DTYPE or input.dim() < 1:
         raise ValueError(f"{what}: input of {FP8_DTYPE} expected, got {tuple(input.shape)} {input.dtype}")
-    if out_dtype not in _DTYPE:
+    code = _DTYPE.get(out_dtype)
+    if code is None:
         raise ValueError(f"{what}: out_dtype {out_dtype}: fp16 and bf16 are supported")
+    dev = input.device
+    lead = input.shape[:-1]
     K = input.shape[-1]
     groups = (K + FP8_GROUP - 1) // FP8_GROUP
-    if scales.dtype != torch.float32 or scales.shape != input.shape[:-1] + (groups,):
-        raise ValueError(f"{what}: scales {tuple(input.shape[:-1]) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
-    weight, weight_scales, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype)
-    N = weight.shape[0]
-    T = input.shape[:-1].numel()
-    out = torch.empty(input.shape[:-1] + (N,), dtype=out_dtype, device=dev)
+    if scales.dtype != torch.float32 or scales.shape != lead + (groups,):
+        raise ValueError(f"{what}: scales {tuple(lead) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
+    weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype, dev)
+    out = weight.new_empty(lead + (N,), dtype=out_dtype)
+    T = lead.numel()
     if T and N:
-        q2 = input if input.dim() == 2 else input.reshape(T, K)
-        if K and (q2.stride(1) != 1 or (T > 1 and q2.stride(0) < K)):
+        q2, s2 = (input, scales) if len(lead) == 1 else (input.reshape(T, K), scales.reshape(T, groups))
+        q0, q1 = q2.stride()
+        if (q1 != 1 and K > 1) or (q0 < K and T > 1):
             q2 = q2.contiguous()
-        s2 = scales if scales.dim() == 2 else scales.reshape(T, groups)
+            q0 = K
+        st, sg = s2.stride()
         nbytes = _fp8_tmp_bytes("pq_fp8_block_gemm_tmp_bytes", T, N, K)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _on_device(dev):
             rc = _lib.load().pq_fp8_block_gemm(
-                q2.data_ptr(), T, q2.stride(0) if T > 1 else K, s2.data_ptr(), s2.stride(0), s2.stride(1),
-                weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(), groups,
-                bias.data_ptr() if bias is not None else None, N, K, _DTYPE[out_dtype], out.data_ptr(), N,
-                tmp.data_ptr() if tmp is not None else None, nbytes, _stream_ptr(dev))
+                q2.data_ptr(), T, q0 if T > 1 else K, s2.data_ptr(), st, sg, weight.data_ptr(), w0, weight_scales.data_ptr(),
+                groups, bptr, N, K, code, out.data_ptr(), N, None if tmp is None else tmp.data_ptr(), nbytes, _stream_ptr(dev))
         if rc:
             _raise(rc)
     return out
@@ -882,21 +905,16 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
 def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                      bias: Optional[torch.Tensor]) -> torch.Tensor:
     what = "fp8_block_linear"
-    dev = _check_device(input, weight, weight_scales, bias)
-    x2, xs = _fp8_input(input, what)
-    T, K = x2.shape
-    weight, weight_scales, bias = _fp8_weight(what, K, weight, weight_scales, bias, input.dtype)
-    N = weight.shape[0]
-    out = torch.empty(input.shape[:-1] + (N,), dtype=input.dtype, device=dev)
+    x2, T, K, xs, dev, code = _fp8_act(input, what)
+    weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, input.dtype, dev)
+    out = input.new_empty((T, N) if input.dim() == 2 else input.shape[:-1] + (N,))
     if T and N:
-        L = _lib.load()
         nbytes = _fp8_tmp_bytes("pq_fp8_block_linear_tmp_bytes", T, N, K)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with _on_device(dev):
-            rc = L.pq_fp8_block_linear(
-                x2.data_ptr(), T, xs, weight.data_ptr(), weight.stride(0) if N > 1 else K, weight_scales.data_ptr(),
-                weight_scales.shape[1], bias.data_ptr() if bias is not None else None, N, K, _DTYPE[input.dtype],
-                out.data_ptr(), N, tmp.data_ptr() if tmp is not None else None, nbytes, _stream_ptr(dev))
+            rc = _lib.load().pq_fp8_block_linear(
+                x2.data_ptr(), T, xs, weight.data_ptr(), w0, weight_scales.data_ptr(), weight_scales.shape[1], bptr, N, K, code,
+                out.data_ptr(), N, None if tmp is None else tmp.data_ptr(), nbytes, _stream_ptr(dev))
         if rc:
             _raise(rc)
     return out
