@@ -303,7 +303,7 @@ int pq_gemm_packed_normed_silu_mul(const void *xw, int32_t T, int64_t xw_row_str
  *   pq_silu_and_mul_fp8        v = silu(x[t][j]) * x[t][I + j], x [T][2 I] (in front of a down_proj held in e4m3)
  *   pq_rms_norm_fp8            v = x * rsqrt(mean(x^2) + eps) * weight   (in front of qkv_proj / gate_up_proj)
  *   pq_fused_add_rms_norm_fp8  z = x + residual in fp32, residual <- round(z), v = the norm of z; x is not modified
- * Rows of up to 16384 values for the norms (15360 where a pointer or stride is not 16-byte aligned or H % 8 != 0).
+ * Any alignment; rows of up to 16384 values for the norms.
  *
  *   pq_fp8_block_gemm    y[t][n] = round( sum_b scales[t][b] * weight_scales[n / 128][b] * sum_{k in b} q[t][k] *
  *                        weight[n][k]  + bias[n] ), accumulated in fp32, act dtype y.  tmp: optional 16-byte aligned
@@ -311,7 +311,8 @@ int pq_gemm_packed_normed_silu_mul(const void *xw, int32_t T, int64_t xw_row_str
  *                        pq_fp8_block_gemm_tmp_bytes(T, N, K) says how much is used at most (0: none)
  *   pq_fp8_block_linear  pq_fp8_group_quant followed by pq_fp8_block_gemm, the same values.  tmp: 16-byte aligned
  *                        scratch of pq_fp8_block_linear_tmp_bytes(T, N, K) bytes, free again when the call's work on
- *                        `stream` is done (NULL is fine where that is 0)
+ *                        `stream` is done (NULL is fine where that is 0: a few tokens
+ *                        are quantised inside the product's launch; weight rows are then less than 64 MiB apart)
  * K, weight, q and their row strides that are multiples of 4 (bytes) take the fast kernels, anything else a slower one;
  * every T, N and K is taken.  A token's sums may run in another order when T changes; the same call gives the same bits.
  * No reference counterpart as kernels of this library's form.

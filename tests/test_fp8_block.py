@@ -130,7 +130,6 @@ def test_norm_refusals_need_no_gpu():
     assert _norm_rc(r=None) == 1 and "residual" in _lib.last_error()
     assert _norm_rc(w=None) == 1 and _norm_rc(rs=100) == 1 and _norm_rc(xs=100) == 1
     assert _norm_rc(H=16392, xs=16392, rs=16392, qs=16392) == 2         # longer than a block holds
-    assert _norm_rc(H=15361, xs=15361, rs=15361, qs=15361) == 2         # unaligned, longer than the LDS row
     assert _norm_rc(T=0) == 0
 
 
@@ -196,7 +195,7 @@ def test_gpu_silu_and_mul_fp8(T, I, dt):
 @gpu
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 @pytest.mark.parametrize("add", [False, True])
-@pytest.mark.parametrize("T,H", SHAPES + [(3, 8192), (2, 12288), (2, 15359)])
+@pytest.mark.parametrize("T,H", SHAPES + [(3, 8192), (2, 12288), (2, 16383)])
 def test_gpu_norm_fp8(T, H, add, dt):
     gen = torch.Generator().manual_seed(3 * T + H)
     x, w = activations(gen, T, H, DT[dt]), (1 + 0.2 * torch.randn(H, generator=gen)).to(DT[dt])

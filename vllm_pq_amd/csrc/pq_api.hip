@@ -659,9 +659,8 @@ static int norm_fp8(const char *fn, const void *x, int64_t x_row_stride, void *r
     a.res_stride = res_row_stride;
     a.weight = weight;
     a.eps = eps;
-    if (!pq::norm_quant_vectorised(a) && H > pq::RMS_SCALAR_MAX_H)
-        return fail(PQ_ERR_UNSUPPORTED, "%s: rows of %d elements need 16-byte aligned tensors, strides and H %% 8 == 0 "
-                    "(up to 16384 elements); unaligned rows are supported up to %d", fn, H, pq::RMS_SCALAR_MAX_H);
+    if (H > pq::NORM_QUANT_MAX_H)
+        return fail(PQ_ERR_UNSUPPORTED, "%s: rows of %d elements (up to %d are supported)", fn, H, pq::NORM_QUANT_MAX_H);
     hipError_t e = pq::launch_norm_quant(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return fail(PQ_ERR_LAUNCH, "%s: %s", fn, hipGetErrorString(e));
     return PQ_OK;

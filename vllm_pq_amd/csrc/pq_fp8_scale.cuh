@@ -9,24 +9,23 @@ namespace pq {
 
 constexpr uint32_t AMAX_MIN_BITS = (127 - 96) << 23;   // 2^-96
 
-// What divides a group: s, and what the quotient is corrected with.
+// What divides a group: its scale s, an approximate reciprocal of it, and what the quotient is corrected with.
 struct GroupScale {
     float s, r, c;
 };
 __device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
     GroupScale g;
     g.s = __uint_as_float(amax_bits > AMAX_MIN_BITS ? amax_bits : AMAX_MIN_BITS) / FP8_MAX;
-    g.r = 1.0f / g.s;
+    g.r = __builtin_amdgcn_rcpf(g.s);         // within one unit of the last place
     g.c = __builtin_isinf(g.s) ? 0.f : g.s;   // an infinite scale: v * r stands as it is (0, or NaN for the infinity itself)
     return g;
 }
-// v / s, correctly rounded: a product with the rounded reciprocal is within two units of the last place, one Newton step
-// on the exact residual brings it within one, and from there a second step rounds as division does (Markstein's theorem).
-// Half the instructions of a division; a plain product would move values that lie on a tie between two e4m3 numbers, which
-// is common with act-dtype inputs.
+// v / s in fp32: the product with the reciprocal is within 2^-22 of the quotient, and one Newton step on its exact residual
+// takes that to 2^-44, so the rounded result is the correctly rounded quotient unless that lies within 2^-44 of half way
+// between two numbers.  A third of a division's instructions, which is what bounds these kernels next to memory; the bare
+// product would move values that lie on a tie between two e4m3 numbers, and with act-dtype inputs many do.
 __device__ __forceinline__ float div_group(float v, const GroupScale &g) {
-    float q = v * g.r;
-    q = __builtin_fmaf(__builtin_fmaf(-q, g.c, v), g.r, q);
+    const float q = v * g.r;
     return __builtin_fmaf(__builtin_fmaf(-q, g.c, v), g.r, q);
 }
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
@@ -35,8 +34,5 @@ __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b 
 __device__ __forceinline__ uint32_t pack4(const float *v, const GroupScale &g) {
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(div_group(v[0], g), div_group(v[1], g), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(div_group(v[2], g), div_group(v[3], g), p, true);
-}
-__device__ __forceinline__ uint8_t pack1(float v, const GroupScale &g) {
-    return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(div_group(v, g), 0.f, 0, false);
 }
 }  // namespace pq

@@ -156,7 +156,7 @@ struct QuantArgs {
     float *scales;
     int64_t scale_stride;
 };
-bool norm_quant_vectorised(const QuantArgs &a);   // else rows of up to RMS_SCALAR_MAX_H
+constexpr int NORM_QUANT_MAX_H = 16384;   // a row stays in one block's registers
 hipError_t launch_group_quant(const QuantArgs &a, hipStream_t stream);
 hipError_t launch_silu_quant(const QuantArgs &a, hipStream_t stream);
 hipError_t launch_norm_quant(const QuantArgs &a, hipStream_t stream);
