@@ -28,6 +28,7 @@ from torch.nn.parameter import Parameter
 from . import ops
 from .compat import (LinearBase, LinearMethodBase, ParallelLMHead, QUANTIZATION_METHODS, QuantizationConfig,
                      VocabParallelEmbedding, register_quantization_config, set_weight_attrs)
+from .fp8 import BlockFP8LinearMethod, is_fp8_module
 
 PQ_METHOD_NAME = "pq"
 
@@ -53,8 +54,11 @@ class PQConfig(QuantizationConfig):
 
     def __init__(self, in_group_size: int = 8, nbits_per_codebook: int = 8, num_codebooks: int = 1,
                  out_group_size: int = 1, lm_head: bool = False, embeddings: bool = False,
-                 release_reference_codes: bool = False) -> None:
+                 release_reference_codes: bool = False, fp8_modules: Optional[List[str]] = None) -> None:
         super().__init__()
+        # Regular expressions of the linear modules that the checkpoint holds as block-scaled e4m3 values instead (key of
+        # the same name in the HF quantization_config); see fp8.py.
+        self.fp8_modules = list(fp8_modules or [])
         # After the load-time re-layout the kernels read only the packed copy of a linear layer's codes; with this
         # key (same name in the HF quantization_config) the reference-layout tensor gives its storage back (shape and
         # dtype stay): half the code bytes of a model, at the price that pq_dequant on such a layer no longer works.
@@ -110,10 +114,13 @@ class PQConfig(QuantizationConfig):
         og = cls.get_from_keys_or(config, ["out_group_size"], 1)
         return cls(d, nbits, m, og, lm_head=cls.get_from_keys_or(config, ["lm_head"], False),
                    embeddings=cls.get_from_keys_or(config, ["embeddings"], False),
-                   release_reference_codes=cls.get_from_keys_or(config, ["release_reference_codes"], False))
+                   release_reference_codes=cls.get_from_keys_or(config, ["release_reference_codes"], False),
+                   fp8_modules=cls.get_from_keys_or(config, ["fp8_modules"], None))
 
-    def get_quant_method(self, layer: torch.nn.Module, prefix: str) -> Optional["PQLinearMethod"]:
+    def get_quant_method(self, layer: torch.nn.Module, prefix: str) -> Optional[LinearMethodBase]:
         if isinstance(layer, LinearBase):
+            if self.fp8_modules and is_fp8_module(prefix, self.fp8_modules):
+                return BlockFP8LinearMethod(self)
             return PQLinearMethod(self)
         if isinstance(layer, ParallelLMHead):
             return PQEmbeddingMethod(self) if self.lm_head_quantized else None

@@ -15,6 +15,8 @@ the row scale is then refitted by least squares against the reconstruction, and 
 are alternated a few more times (`refits`) from the centroids already found.  Everything runs in torch on the
 device of the weight, so a GPU is used when the weight is on one; there is no dependence on the kernels.
 
+Modules named for it are written as block-scaled e4m3 values instead (fp8.py).
+
 This is tooling beside the hot path: the reference ships no quantiser (its AQLM checkpoints come from a
 separate project), so there is no reference code this restates.
 """
@@ -25,6 +27,7 @@ from typing import Dict, Iterable, List, Optional, Tuple
 
 import torch
 
+from .fp8 import fp8_quantize_weight, fp8_reconstruct
 from .pq import get_int_dtype
 
 __all__ = ["pq_quantize_weight", "pq_reconstruct", "quantize_state_dict", "save_pq_checkpoint", "quantization_config"]
@@ -134,29 +137,41 @@ def pq_reconstruct(codes: torch.Tensor, codebooks: torch.Tensor, scales: torch.T
     return w.reshape(N, G * d) * scales.view(N, 1).to(torch.float32)
 
 
-def quantization_config(d: int, nbits: int, num_codebooks: int = 1) -> Dict[str, int]:
+def quantization_config(d: int, nbits: int, num_codebooks: int = 1, fp8_modules: Optional[List[str]] = None) -> Dict[str, object]:
     """The `quantization_config` entry of the HF config.json that selects this method (PQConfig.from_config)."""
-    return {"quant_method": "pq", "in_group_size": d, "nbits_per_codebook": nbits,
-            "num_codebooks": num_codebooks, "out_group_size": 1}
+    cfg: Dict[str, object] = {"quant_method": "pq", "in_group_size": d, "nbits_per_codebook": nbits,
+                              "num_codebooks": num_codebooks, "out_group_size": 1}
+    if fp8_modules:
+        cfg["fp8_modules"] = list(fp8_modules)
+    return cfg
 
 
 def quantize_state_dict(state: Dict[str, torch.Tensor], include: str = r".*(q_proj|k_proj|v_proj|o_proj|gate_proj|"
                         r"up_proj|down_proj|out_proj|fc1|fc2)\.weight$", d: int = 8, nbits: int = 8,
                         num_codebooks: int = 1, iters: int = 25, seed: int = 0, device: Optional[str] = None,
-                        report: Optional[List[Tuple[str, float]]] = None) -> Dict[str, torch.Tensor]:
+                        report: Optional[List[Tuple[str, float]]] = None,
+                        fp8_modules: Optional[List[str]] = None) -> Dict[str, torch.Tensor]:
     """Replace every `<module>.weight` whose name matches `include` by `<module>.codes/.codebooks/.scales`
     (the checkpoint names the reference's model loaders expect, vllm/model_executor/models/llama.py:371-433);
-    other tensors pass through.  `report` collects (name, relative Frobenius error)."""
+    other tensors pass through.  Modules that one of the `fp8_modules` expressions is found in become
+    `<module>.weight` (e4m3) / `.weight_scale_inv` instead.  `report` collects (name, relative Frobenius error)."""
     pat = re.compile(include)
     out: Dict[str, torch.Tensor] = {}
     for i, (name, t) in enumerate(state.items()):
-        if t.dim() == 2 and pat.match(name) and t.shape[1] % d == 0:
+        base = name[:-len(".weight")]
+        if t.dim() == 2 and pat.match(name) and any(re.search(p, base) for p in fp8_modules or ()):
+            w = t.to(device) if device else t
+            q, scale = fp8_quantize_weight(w)
+            if report is not None:
+                err = (fp8_reconstruct(q, scale) - w.float()).norm() / w.float().norm().clamp_min(1e-30)
+                report.append((name, float(err)))
+            out[name], out[base + ".weight_scale_inv"] = q.cpu(), scale.cpu()
+        elif t.dim() == 2 and pat.match(name) and t.shape[1] % d == 0:
             w = t.to(device) if device else t
             codes, cb, sc = pq_quantize_weight(w, d, nbits, num_codebooks, iters, seed + i)
             if report is not None:
                 err = (pq_reconstruct(codes, cb, sc) - w.float()).norm() / w.float().norm().clamp_min(1e-30)
                 report.append((name, float(err)))
-            base = name[:-len(".weight")]
             out[base + ".codes"], out[base + ".codebooks"], out[base + ".scales"] = codes.cpu(), cb.cpu(), sc.cpu()
         else:
             out[name] = t
@@ -164,13 +179,13 @@ def quantize_state_dict(state: Dict[str, torch.Tensor], include: str = r".*(q_pr
 
 
 def save_pq_checkpoint(state: Dict[str, torch.Tensor], out_dir: str, d: int, nbits: int, num_codebooks: int = 1,
-                       base_config: Optional[dict] = None) -> None:
+                       base_config: Optional[dict] = None, fp8_modules: Optional[List[str]] = None) -> None:
     """Write `model.safetensors` and a `config.json` carrying the quantization_config into `out_dir`."""
     from safetensors.torch import save_file
     os.makedirs(out_dir, exist_ok=True)
     save_file({k: v.contiguous() for k, v in state.items()}, os.path.join(out_dir, "model.safetensors"))
     cfg = dict(base_config or {})
-    cfg["quantization_config"] = quantization_config(d, nbits, num_codebooks)
+    cfg["quantization_config"] = quantization_config(d, nbits, num_codebooks, fp8_modules)
     with open(os.path.join(out_dir, "config.json"), "w") as f:
         json.dump(cfg, f, indent=1)
 
@@ -185,6 +200,8 @@ def _main(argv: Optional[Iterable[str]] = None) -> int:
     ap.add_argument("--nbits", type=int, default=8)
     ap.add_argument("--num-codebooks", type=int, default=1)
     ap.add_argument("--iters", type=int, default=25)
+    ap.add_argument("--fp8", action="append", default=[], metavar="REGEX",
+                    help="keep modules whose name contains this expression in block-scaled e4m3 (may be given again)")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     args = ap.parse_args(argv)
     files = [args.input] if args.input.endswith(".safetensors") else \
@@ -199,10 +216,10 @@ def _main(argv: Optional[Iterable[str]] = None) -> int:
             base_cfg = json.load(f)
     report: List[Tuple[str, float]] = []
     q = quantize_state_dict(state, d=args.sub_dim, nbits=args.nbits, num_codebooks=args.num_codebooks,
-                            iters=args.iters, device=args.device, report=report)
+                            iters=args.iters, device=args.device, report=report, fp8_modules=args.fp8)
     for name, err in report:
         print(f"{name}: relative error {err:.4f}")
-    save_pq_checkpoint(q, args.output, args.sub_dim, args.nbits, args.num_codebooks, base_cfg)
+    save_pq_checkpoint(q, args.output, args.sub_dim, args.nbits, args.num_codebooks, base_cfg, args.fp8)
     return 0
 
 
