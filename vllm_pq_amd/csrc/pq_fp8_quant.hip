@@ -33,8 +33,15 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
     return umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
 }
 
-// silu(g) * u in fp32, a few units of the last place from it (an 8-bit value has room for 2^20 of them)
-__device__ __forceinline__ float silu_mul(float g, float u) { return g * __builtin_amdgcn_rcpf(1.0f + __expf(-g)) * u; }
+// silu(g) * u in fp32, about a unit of the last place off.  exp(-g) as 2^t, t = -g log2(e): what t's rounding leaves out (up
+// to |t| 2^-24 of the result) is put back to first order; the reciprocal gets one Newton step.  Below -87 the exponential
+// stands still (silu is under 2^-118 there), so no infinity comes up that g does not bring.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+    constexpr float L = 1.4426950408889634f, L_LO = (float)(1.4426950408889634074 - (double)L), LN2 = 0.6931471805599453f;
+    const float x = fmaxf(g, -87.0f), t = -x * L, rest = __builtin_fmaf(-x, L_LO, __builtin_fmaf(-x, L, -t));
+    const float p = __builtin_amdgcn_exp2f(t), d = 1.0f + __builtin_fmaf(p * rest, LN2, p), r = __builtin_amdgcn_rcpf(d);
+    return g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) * u;
+}
 
 // 8 act-dtype values from any address; WHOLE: all of a row's pieces have 8, else the first `valid` and zeros behind, nothing
 // read behind them.  ONCE: no one reads them again (past the caches)

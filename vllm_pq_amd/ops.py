@@ -777,15 +777,23 @@ def _fp8_act(input: torch.Tensor, what: str):
 def _fp8_outputs(input: torch.Tensor, T: int, H: int, dev):
     """(q [..., H], scales [..., groups] over [groups][T] storage)."""
     groups = (H + FP8_GROUP - 1) // FP8_GROUP
+    q = torch.empty_strided((T, H), (H, 1), dtype=FP8_DTYPE, device=dev)
     s = torch.empty_strided((T, groups), (1, T), dtype=torch.float32, device=dev)
     if input.dim() == 2:
-        return input.new_empty((T, H), dtype=FP8_DTYPE), s
+        return q, s
     lead = input.shape[:-1]
-    return input.new_empty(lead + (H,), dtype=FP8_DTYPE), s.reshape(lead + (groups,))
+    return q.view(lead + (H,)), s.reshape(lead + (groups,))
 
 
-def _on_current(dev) -> bool:
-    return dev.index == torch.cuda.current_device()
+def _call_on(dev, fn, *args) -> None:
+    """fn(*args, stream) on `dev`, with the current stream of that device; raises what the library reports."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, _stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream_ptr(dev))
+    if rc:
+        _raise(rc)
 
 
 def _fp8_quant_impl(fn: str, input: torch.Tensor, halves: int):
@@ -795,14 +803,7 @@ def _fp8_quant_impl(fn: str, input: torch.Tensor, halves: int):
         raise ValueError(f"{fn[3:]}: input {tuple(input.shape)} does not halve")
     q, s = _fp8_outputs(input, T, H, dev)
     if T and H:
-        call = getattr(_lib.load(), fn)
-        if _on_current(dev):
-            rc = call(x2.data_ptr(), xs, T, H, code, q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
-        else:
-            with _on_device(dev):
-                rc = call(x2.data_ptr(), xs, T, H, code, q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
-        if rc:
-            _raise(rc)
+        _call_on(dev, getattr(_lib.load(), fn), x2.data_ptr(), xs, T, H, code, q.data_ptr(), H, s.data_ptr(), T)
     return q, s
 
 
@@ -816,20 +817,16 @@ def _fp8_norm_impl(input: torch.Tensor, residual: Optional[torch.Tensor], weight
     if weight.shape != (H,) or (residual is not None and residual.shape != input.shape):
         raise ValueError(f"{what}: shapes {tuple(input.shape)}"
                          f"{'' if residual is None else f' / {tuple(residual.shape)}'}, weight {tuple(weight.shape)}")
-    r2, rs = _rows(residual, f"{what} residual") if residual is not None and T and H else (None, 0)
     q, s = _fp8_outputs(input, T, H, dev)
     if T and H:
         w = weight if weight.is_contiguous() else weight.contiguous()
-        L = _lib.load()
-        with _on_device(dev):
-            if r2 is None:
-                rc = L.pq_rms_norm_fp8(x2.data_ptr(), xs, w.data_ptr(), epsilon, T, H, code, q.data_ptr(), H, s.data_ptr(), T,
-                                       _stream_ptr(dev))
-            else:
-                rc = L.pq_fused_add_rms_norm_fp8(x2.data_ptr(), xs, r2.data_ptr(), rs, w.data_ptr(), epsilon, T, H, code,
-                                                 q.data_ptr(), H, s.data_ptr(), T, _stream_ptr(dev))
-        if rc:
-            _raise(rc)
+        if residual is None:
+            _call_on(dev, _lib.load().pq_rms_norm_fp8, x2.data_ptr(), xs, w.data_ptr(), epsilon, T, H, code, q.data_ptr(), H,
+                     s.data_ptr(), T)
+        else:
+            r2, rs = (residual, H) if residual.is_contiguous() else _rows(residual, f"{what} residual")
+            _call_on(dev, _lib.load().pq_fused_add_rms_norm_fp8, x2.data_ptr(), xs, r2.data_ptr(), rs, w.data_ptr(), epsilon, T, H,
+                     code, q.data_ptr(), H, s.data_ptr(), T)
     return q, s
 
 
@@ -840,24 +837,29 @@ def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Te
     if weight.device != dev or weight_scales.device != dev or (bias is not None and bias.device != dev):
         _check_device(weight, weight_scales, bias)
         raise RuntimeError(f"{what}: weight on {weight.device}, activations on {dev}")
-    if weight.dtype != FP8_DTYPE or weight.dim() != 2 or weight.shape[1] != K:
-        raise ValueError(f"{what}: weight [out_features, {K}] of {FP8_DTYPE} expected, got {tuple(weight.shape)} {weight.dtype}")
-    N = weight.shape[0]
+    shape = weight.shape
+    if weight.dtype is not FP8_DTYPE or len(shape) != 2 or shape[1] != K:
+        raise ValueError(f"{what}: weight [out_features, {K}] of {FP8_DTYPE} expected, got {tuple(shape)} {weight.dtype}")
+    N = shape[0]
     blocks = ((N + FP8_GROUP - 1) // FP8_GROUP, (K + FP8_GROUP - 1) // FP8_GROUP)
-    if weight_scales.dtype != torch.float32 or weight_scales.shape != blocks:
+    if weight_scales.dtype is not torch.float32 or weight_scales.shape != blocks:
         raise ValueError(f"{what}: weight_scales {blocks} fp32 expected (one per 128 x 128 block), got "
                          f"{tuple(weight_scales.shape)} {weight_scales.dtype}")
+    bptr = None
     if bias is not None:
-        if bias.numel() != N or bias.dtype != dtype:
+        if bias.numel() != N or bias.dtype is not dtype:
             raise ValueError(f"{what}: bias must hold one value of {dtype} per output row")
         bias = bias.reshape(-1).contiguous()
-    w0, w1 = weight.stride()
-    if (w1 != 1 and K > 1) or (w0 < K and N > 1):
-        weight = weight.contiguous()
-        w0 = K
+        bptr = bias.data_ptr()
+    w0 = K
+    if not weight.is_contiguous():
+        w0, w1 = weight.stride()
+        if (w1 != 1 and K > 1) or (w0 < K and N > 1):
+            weight = weight.contiguous()
+            w0 = K
     if not weight_scales.is_contiguous():
         weight_scales = weight_scales.contiguous()
-    return weight, (w0 if N > 1 else K), N, weight_scales, (None if bias is None else bias.data_ptr()), bias
+    return weight, (w0 if N > 1 else K), N, weight_scales, bptr, bias
 
 
 @functools.lru_cache(maxsize=4096)
@@ -882,8 +884,10 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
     if scales.dtype != torch.float32 or scales.shape != lead + (groups,):
         raise ValueError(f"{what}: scales {tuple(lead) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
     weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype, dev)
-    out = weight.new_empty(lead + (N,), dtype=out_dtype)
     T = lead.numel()
+    out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=dev)
+    if len(lead) != 1:
+        out = out.view(lead + (N,))
     if T and N:
         q2, s2 = (input, scales) if len(lead) == 1 else (input.reshape(T, K), scales.reshape(T, groups))
         q0, q1 = q2.stride()
@@ -893,12 +897,9 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
         st, sg = s2.stride()
         nbytes = _fp8_tmp_bytes("pq_fp8_block_gemm_tmp_bytes", T, N, K)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with _on_device(dev):
-            rc = _lib.load().pq_fp8_block_gemm(
-                q2.data_ptr(), T, q0 if T > 1 else K, s2.data_ptr(), st, sg, weight.data_ptr(), w0, weight_scales.data_ptr(),
-                groups, bptr, N, K, code, out.data_ptr(), N, None if tmp is None else tmp.data_ptr(), nbytes, _stream_ptr(dev))
-        if rc:
-            _raise(rc)
+        _call_on(dev, _lib.load().pq_fp8_block_gemm, q2.data_ptr(), T, q0 if T > 1 else K, s2.data_ptr(), st, sg,
+                 weight.data_ptr(), w0, weight_scales.data_ptr(), groups, bptr, N, K, code, out.data_ptr(), N,
+                 None if tmp is None else tmp.data_ptr(), nbytes)
     return out
 
 
@@ -907,16 +908,15 @@ def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: t
     what = "fp8_block_linear"
     x2, T, K, xs, dev, code = _fp8_act(input, what)
     weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, input.dtype, dev)
-    out = input.new_empty((T, N) if input.dim() == 2 else input.shape[:-1] + (N,))
+    out = torch.empty_strided((T, N), (N, 1), dtype=input.dtype, device=dev)
+    if input.dim() != 2:
+        out = out.view(input.shape[:-1] + (N,))
     if T and N:
         nbytes = _fp8_tmp_bytes("pq_fp8_block_linear_tmp_bytes", T, N, K)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with _on_device(dev):
-            rc = _lib.load().pq_fp8_block_linear(
-                x2.data_ptr(), T, xs, weight.data_ptr(), w0, weight_scales.data_ptr(), weight_scales.shape[1], bptr, N, K, code,
-                out.data_ptr(), N, None if tmp is None else tmp.data_ptr(), nbytes, _stream_ptr(dev))
-        if rc:
-            _raise(rc)
+        _call_on(dev, _lib.load().pq_fp8_block_linear, x2.data_ptr(), T, xs, weight.data_ptr(), w0, weight_scales.data_ptr(),
+                 (K + FP8_GROUP - 1) // FP8_GROUP, bptr, N, K, code, out.data_ptr(), N, None if tmp is None else tmp.data_ptr(),
+                 nbytes)
     return out
 
 
