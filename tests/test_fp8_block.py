@@ -331,6 +331,54 @@ def test_gpu_block_gemm_tiles(T, N, K):
 
 
 @gpu
+@pytest.mark.parametrize("T,N,K", [(17, 130, 18), (40, 257, 1001), (300, 700, 4099), (1000, 520, 2001), (64, 512, 8195), (200, 30, 15), (33, 5, 127)])
+def test_gpu_block_gemm_any_length(T, N, K):
+    """A K that is no multiple of 4: with the scratch (operands laid out there), without it, and with rows inside wider ones."""
+    gen = torch.Generator().manual_seed(T + N + K)
+    q, s = ops.fp8_group_quant(activations(gen, T, K, torch.float16).to(DEV))
+    w, ws = (t.to(DEV) for t in weight(gen, N, K))
+    bias = torch.randn(N, generator=gen).to(torch.float16).to(DEV)
+    y = ops.fp8_block_gemm(q, s, w, ws, bias, torch.float16)
+    check_gemm(y, q, s, w, ws, bias, DEV)
+    # around each row of both operands: bytes that are NaN as e4m3
+    qw, ww = (torch.full((t.shape[0] + 2, K + 21), 0x7f, dtype=torch.uint8, device=DEV) for t in (q, w))
+    qw[1:-1, 9:K + 9], ww[1:-1, 9:K + 9] = q.view(torch.uint8), w.view(torch.uint8)
+    args = (qw[1:-1, 9:K + 9].view(F8), s, ww[1:-1, 9:K + 9].view(F8), ws, bias, torch.float16)
+    assert torch.equal(y, ops.fp8_block_gemm(*args))
+    z = torch.empty_like(y)
+    tmp = torch.full((ops._fp8_tmp_bytes("pq_fp8_block_gemm_tmp_bytes", T, N, K) + 64,), 0x7f, dtype=torch.uint8, device=DEV)
+    for scratch in (0, 16, tmp.numel() - 64):       # none, too little, what is asked for
+        z.zero_()
+        assert _lib.load().pq_fp8_block_gemm(args[0].data_ptr(), T, K + 21, s.data_ptr(), 1, T, args[2].data_ptr(), K + 21, ws.data_ptr(),
+                                             blocks(K), bias.data_ptr(), N, K, 0, z.data_ptr(), N, tmp.data_ptr() if scratch else None,
+                                             scratch, torch.cuda.current_stream().cuda_stream) == 0
+        check_gemm(z, q, s, w, ws, bias, DEV)
+        assert (tmp[-64:] == 0x7f).all()
+    assert torch.equal(y, z)
+
+
+@gpu
+@pytest.mark.parametrize("T,N,K", [(4, 40, 300), (4, 40, 4096 + 300), (40, 64, 384), (40, 64, 131), (300, 200, 640), (300, 4096, 1152)])
+def test_gpu_gemm_infinite_scales(T, N, K):
+    """An infinite scale of a token's (row block's) last group and finite values: the sums are infinite, with the values' sign,
+    also where a wave has no group of its own behind it."""
+    q = torch.ones(T, K, device=DEV).to(F8)
+    w = torch.ones(N, K, device=DEV).to(F8)
+    w[1::2] = torch.full((), -1.0).to(F8)
+    s, ws = torch.ones(T, blocks(K), device=DEV), torch.ones(blocks(N), blocks(K), device=DEV)
+    sign = torch.ones(N, device=DEV)
+    sign[1::2] = -1
+    s[1::2, -1] = math.inf
+    y = ops.fp8_block_gemm(q, s, w, ws).float()
+    assert torch.equal(y[1::2], (sign * math.inf).expand(T // 2, N))
+    assert torch.isfinite(y[::2]).all()
+    ws[0, -1] = math.inf
+    y = ops.fp8_block_gemm(q, s, w, ws).float()
+    assert torch.equal(y[:, :128], (sign[:128] * math.inf).expand(T, min(N, 128)))
+    assert torch.isfinite(y[::2, 128:]).all()
+
+
+@gpu
 def test_gpu_matrix_instruction():
     """What the tolerance of the products rests on, seen through the operator: 448 * 448 and its negative cancel, and what is
     left of a small product tells how it was held.  A lane holds 32 of the block's features, in groups of 8."""

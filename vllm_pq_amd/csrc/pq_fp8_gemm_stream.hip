@@ -122,7 +122,6 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
     }
 #pragma unroll
     for (int i = 0; i < SM_KPW; ++i) {
-        if (kb0 + SM_WAVES * i >= kb_end) xs[i] = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) xv[i][e] &= keep(i, e >> 2, e & 3);
     }
@@ -140,7 +139,7 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
 #pragma unroll
         for (int i = 0; i < SM_KPW; ++i) {
             const f32x4 p = mfma_block(wv[now][i], xv[i]);
-            const float s = xs[i] * ws[block(i)];
+            const float s = kb0 + SM_WAVES * i < kb_end ? xs[i] * ws[block(i)] : 0.f;   // (no 0 x infinity behind the range)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(s, p[e], acc[e]);
         }

@@ -151,6 +151,9 @@ __global__ __launch_bounds__(WN * WT * KG * 64) void fp8_gemm_tiled_kernel(Fp8Ge
 #pragma unroll
             for (int j = 0; j < TF; ++j) xv[j][e] &= keep;
         }
+#pragma unroll
+        for (int j = 0; j < TF; ++j) xs_next[j] = kb < k_end ? xs_next[j] : 0.f;   // (no 0 x infinity behind the end)
+        ws_next = kb < k_end ? ws_next : 0.f;
     };
     auto scales = [&](int st) {
         const unsigned char *f = stages + (st % STAGES) * C::STAGE;
