@@ -119,6 +119,13 @@ def test_quant_refusals_need_no_gpu():
     assert _quant_rc("pq_silu_and_mul_fp8", xs=255) == 1                # the input row is twice as long
 
 
+def test_rows_that_do_not_fit_the_index_are_refused():
+    big = 2 ** 31 - 1
+    assert _quant_rc("pq_fp8_group_quant", H=big, xs=big, qs=big) == 2 and "elements" in _lib.last_error()
+    assert _norm_rc(H=big, xs=big, rs=big, qs=big) == 2
+    assert _gemm_rc(N=big, ys=big) == 1 and _gemm_rc(K=big, qs=big, wst=big, wss=big) == 1
+
+
 def _norm_rc(**kw):
     a = dict(x=256, xs=128, r=256, rs=128, w=256, T=4, H=128, dtype=1, q=256, qs=128, s=256, ss=4)
     a.update(kw)
@@ -443,6 +450,59 @@ def test_gpu_gemm_leaves_what_is_outside_its_rows(T):
         assert rc == 0
         assert (y[T:] == 31).all() and (y[:, cols:] == 31).all()
         check_gemm(y[:T, :cols], q, s, w[:cols], ws[:blocks(cols)], None)
+
+
+@gpu
+@pytest.mark.parametrize("T,N,stride", [(600, 520, 2 ** 23 - 128), (600, 520, 2 ** 23 + 128), (16, 600, 2 ** 23), (5, 72, 2 ** 26 - 64),
+                                        (3, 33, 2 ** 27)])
+def test_gpu_offsets_past_32_bits(T, N, stride):
+    """Rows so far apart that the last ones lie more than 2^32 elements behind the first: weights, outputs and, for many tokens,
+    activations."""
+    K = 272
+    gen = torch.Generator().manual_seed(N)
+    x = activations(gen, T, K, torch.bfloat16).to(DEV)
+    q, s = ops.fp8_group_quant(x)
+    w, ws = (t.to(DEV) for t in weight(gen, N, K))
+
+    def spread(t):
+        rows = torch.empty(t.shape[0] * stride, dtype=t.dtype, device=DEV).view(t.shape[0], stride)[:, :t.shape[1]]
+        return rows.copy_(t) if t.dtype != F8 else rows.view(torch.uint8).copy_(t.view(torch.uint8)).view(F8)
+    far = spread(w)
+    check_gemm(ops.fp8_block_gemm(q, s, far, ws), q, s, w, ws, None, DEV)
+    del far
+    if T > 16:
+        far = spread(q)
+        check_gemm(ops.fp8_block_gemm(far, s, w, ws), q, s, w, ws, None, DEV)
+        del far
+        far = spread(x)
+        q2, s2 = ops.fp8_group_quant(far)
+        assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
+        check_gemm(ops.fp8_block_linear(far, w, ws), q, s, w, ws, None, DEV)
+        one = torch.ones(K, dtype=x.dtype, device=DEV)
+        for a, b in zip(ops.rms_norm_fp8(far, one, 1e-5), ops.rms_norm_fp8(x, one, 1e-5)):
+            assert torch.equal(a.float(), b.float())
+        del far
+    y = torch.empty(T * stride, dtype=torch.bfloat16, device=DEV).view(T, stride)[:, :N]
+    assert _lib.load().pq_fp8_block_gemm(q.data_ptr(), T, K, s.data_ptr(), 1, T, w.data_ptr(), K, ws.data_ptr(), 3, None, N, K, 1,
+                                         y.data_ptr(), stride, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    check_gemm(y.contiguous(), q, s, w, ws, None, DEV)
+
+
+@gpu
+@pytest.mark.parametrize("T", [3, 16, 40, 300])
+@pytest.mark.parametrize("K", [256, 384, 1027, 4500])
+def test_gpu_a_token_stands_for_itself(T, K):
+    """A padding row of infinities or NaN leaves the other tokens' outputs as they were, bit for bit."""
+    gen = torch.Generator().manual_seed(T + K)
+    N = 200
+    x = activations(gen, T, K, torch.bfloat16).to(DEV)
+    w, ws = (t.to(DEV) for t in weight(gen, N, K))
+    y, z = ops.fp8_block_linear(x, w, ws), ops.fp8_block_gemm(*ops.fp8_group_quant(x), w, ws)
+    for bad in (math.nan, math.inf):
+        x[1] = bad
+        rest = [t for t in range(T) if t != 1]
+        for got, want in ((ops.fp8_block_linear(x, w, ws), y), (ops.fp8_block_gemm(*ops.fp8_group_quant(x), w, ws), z)):
+            assert torch.equal(got[rest], want[rest]) and got[1].isnan().all()
 
 
 @gpu

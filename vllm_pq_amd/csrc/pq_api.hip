@@ -612,6 +612,7 @@ static int fill_quant(pq::QuantArgs &a, const char *fn, const void *x, int64_t x
     int rc = check_rows(fn, T, H, dtype);
     if (rc) return rc;
     a = pq::QuantArgs{x, x_row_stride, nullptr, 0, nullptr, 0.f, T, H, dtype, q, q_row_stride, scales, scale_group_stride};
+    if (H > INT32_MAX - 4096) return fail(PQ_ERR_UNSUPPORTED, "%s: rows of %d elements", fn, H);
     if (T == 0 || H == 0) return PQ_OK;
     if (!x || !q || !scales) return fail(PQ_ERR_INVALID_ARGUMENT, "%s: NULL tensor pointer", fn);
     if (x_row_stride < x_row || q_row_stride < H)

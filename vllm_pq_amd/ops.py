@@ -767,6 +767,8 @@ def _fp8_act(input: torch.Tensor, what: str):
     else:
         x2 = input
         T, H = input.shape
+    if (T | H) >> 31:
+        raise ValueError(f"{what}: input {tuple(input.shape)}: sizes below 2^31 are supported")
     s0, s1 = x2.stride()
     if (s1 != 1 and H > 1) or (s0 < H and T > 1):
         x2 = x2.contiguous()
@@ -841,6 +843,8 @@ def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Te
     if weight.dtype is not FP8_DTYPE or len(shape) != 2 or shape[1] != K:
         raise ValueError(f"{what}: weight [out_features, {K}] of {FP8_DTYPE} expected, got {tuple(shape)} {weight.dtype}")
     N = shape[0]
+    if (N | K) >> 31:
+        raise ValueError(f"{what}: weight {tuple(shape)}: sizes below 2^31 are supported")
     blocks = ((N + FP8_GROUP - 1) // FP8_GROUP, (K + FP8_GROUP - 1) // FP8_GROUP)
     if weight_scales.dtype is not torch.float32 or weight_scales.shape != blocks:
         raise ValueError(f"{what}: weight_scales {blocks} fp32 expected (one per 128 x 128 block), got "
@@ -885,6 +889,8 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
         raise ValueError(f"{what}: scales {tuple(lead) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
     weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype, dev)
     T = lead.numel()
+    if T >> 31:
+        raise ValueError(f"{what}: {T} tokens: sizes below 2^31 are supported")
     out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=dev)
     if len(lead) != 1:
         out = out.view(lead + (N,))
