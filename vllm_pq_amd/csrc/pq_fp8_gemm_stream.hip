@@ -20,10 +20,12 @@
 
 namespace pq {
 
-constexpr int SM_WAVES = 8, SM_KPW = 4, SM_ROW = 20;   // waves; scale blocks of a wave; floats between tokens' sums
+constexpr int SM_WAVES = 8, SM_KPW = 4, SM_ROW = 20;   // waves; scale blocks of a wave at most; floats between tokens' sums
 constexpr int SM_RANGE = SM_WAVES * SM_KPW;            // scale blocks of a range of K
 constexpr size_t SM_SUM_BYTES = 2 * SM_WAVES * 16 * SM_ROW * sizeof(float);
 constexpr int SM_MAX_FUSED = 8192;                     // values a block quantises at most (8.5 KiB of LDS)
+
+typedef __attribute__((address_space(4))) float const_float;   // memory that no kernel running writes
 
 // 16 bytes from any address: one load, whatever the alignment
 __device__ __forceinline__ u32x4 load16u(const uint8_t *p) {
@@ -33,7 +35,7 @@ __device__ __forceinline__ u32x4 load16u(const uint8_t *p) {
 }
 
 // part: NULL, or the ranges' sums [gridDim.y][T][np]
-template <typename AT, bool FUSED>
+template <typename AT, bool FUSED, int KPW>
 __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8GemmArgs a, int tiles, int range, float *part, int64_t np) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     float *const s_sum = reinterpret_cast<float *>(smem);
@@ -60,18 +62,19 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
         const uint8_t *base = w + (int64_t)tile * 16 * a.w_stride;
         const uint32_t row = (uint32_t)min(r, a.N - 1 - tile * 16) * (uint32_t)a.w_stride;
 #pragma unroll
-        for (int i = 0; i < SM_KPW; ++i) {
+        for (int i = 0; i < KPW; ++i) {
             const uint8_t *bk = base + block(i) * FP8_GROUP;
             to[i] = join(load16u(bk + (row + piece(i, 0))), load16u(bk + (row + piece(i, 1))));
         }
     };
-    i32x8 wv[2][SM_KPW];
+    i32x8 wv[2][KPW];
     int tile = blockIdx.x;
     load(tile, wv[0]);
 
     // ---- the activations of this wave's scale blocks
-    i32x8 xv[SM_KPW];
-    float xs[SM_KPW];
+    i32x8 xv[KPW];
+    float xs[KPW];
+    uint32_t own[KPW];
     if constexpr (FUSED) {
         // 32 lanes x 4 values take a group
         uint8_t *const s_q = smem + SM_SUM_BYTES;
@@ -105,7 +108,7 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
         __syncthreads();
         const int t = min(r, a.T - 1);
 #pragma unroll
-        for (int i = 0; i < SM_KPW; ++i) {
+        for (int i = 0; i < KPW; ++i) {
             const uint8_t *row = s_q + (t * KB + block(i)) * FP8_GROUP - 16;
             xv[i] = join(*reinterpret_cast<const u32x4 *>(row + piece(i, 0)), *reinterpret_cast<const u32x4 *>(row + piece(i, 1)));
             xs[i] = s_s[t * KB + block(i)];
@@ -114,14 +117,16 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
         const int t = min(r, a.T - 1);
         const uint8_t *row = static_cast<const uint8_t *>(a.q) + (int64_t)t * a.q_stride - 16;
 #pragma unroll
-        for (int i = 0; i < SM_KPW; ++i) {
+        for (int i = 0; i < KPW; ++i) {
             const uint8_t *bk = row + block(i) * FP8_GROUP;
             xv[i] = join(load16u(bk + piece(i, 0)), load16u(bk + piece(i, 1)));
             xs[i] = a.xs[t * a.xs_token + block(i) * a.xs_group];
         }
     }
 #pragma unroll
-    for (int i = 0; i < SM_KPW; ++i) {
+    for (int i = 0; i < KPW; ++i) {
+        own[i] = kb0 + SM_WAVES * i < kb_end ? ~0u : 0u;   // scales behind the range count as 0 (no 0 x infinity)
+        asm("" : "+v"(own[i]));                            // (a mask: no branch around a load)
 #pragma unroll
         for (int e = 0; e < 8; ++e) xv[i][e] &= keep(i, e >> 2, e & 3);
     }
@@ -133,13 +138,17 @@ __global__ __launch_bounds__(SM_WAVES * 64, 4) void fp8_gemm_stream_kernel(Fp8Ge
         constexpr int now = decltype(now_t)::value;           // buffer of this tile's weights
         constexpr bool more = decltype(more_t)::value;        // there is a next tile
         const int next = tile + gridDim.x;
-        const float *ws = a.ws + (int64_t)(tile * 16 / FP8_GROUP) * a.ws_stride;
+        // read through the scalar cache: a load per wave and not per lane, asked for before the next weights
+        const const_float *ws = (const const_float *)(uintptr_t)(a.ws + (int64_t)(tile * 16 / FP8_GROUP) * a.ws_stride);
+        float wscale[KPW];
+#pragma unroll
+        for (int i = 0; i < KPW; ++i) wscale[i] = ws[block(i)];
         f32x4 acc{0.f, 0.f, 0.f, 0.f};
         if (more) load(next, wv[now ^ 1]);
 #pragma unroll
-        for (int i = 0; i < SM_KPW; ++i) {
+        for (int i = 0; i < KPW; ++i) {
             const f32x4 p = mfma_block(wv[now][i], xv[i]);
-            const float s = kb0 + SM_WAVES * i < kb_end ? xs[i] * ws[block(i)] : 0.f;   // (no 0 x infinity behind the range)
+            const float s = __uint_as_float(__float_as_uint(xs[i] * wscale[i]) & own[i]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(s, p[e], acc[e]);
         }
@@ -180,8 +189,14 @@ static hipError_t stream_at(const Fp8GemmArgs &a, hipStream_t stream) {
     const int tiles = (a.N + 15) / 16, slots = 512 / ranges;   // two blocks a CU, each with every so-manieth tile
     const int64_t np = ((int64_t)a.N + 3) / 4 * 4;
     float *part = ranges > 1 ? static_cast<float *>(a.tmp) : nullptr;
-    hipLaunchKernelGGL((fp8_gemm_stream_kernel<AT, FUSED>), dim3((unsigned)(tiles < slots ? tiles : slots), (unsigned)ranges),
-                       dim3(SM_WAVES * 64), lds, stream, a, tiles, range, part, np);
+    const dim3 grid((unsigned)(tiles < slots ? tiles : slots), (unsigned)ranges);
+    // as many blocks of K per wave as there are: those behind the end are fetched and multiplied all the same.  With 4 always:
+    // 16 tokens of 4096 x 1000 5.2 us against 4.0, 8 of 4096 x 2048 6.3 against 5.3, 1 of 8192 x 1536 8.6 against 6.3
+    auto kern = range <= SM_WAVES       ? fp8_gemm_stream_kernel<AT, FUSED, 1>
+                : range <= 2 * SM_WAVES ? fp8_gemm_stream_kernel<AT, FUSED, 2>
+                : range <= 3 * SM_WAVES ? fp8_gemm_stream_kernel<AT, FUSED, 3>
+                                        : fp8_gemm_stream_kernel<AT, FUSED, SM_KPW>;
+    hipLaunchKernelGGL(kern, grid, dim3(SM_WAVES * 64), lds, stream, a, tiles, range, part, np);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess || !part ? e : launch_fp8_join(a, part, ranges, np, stream);
 }

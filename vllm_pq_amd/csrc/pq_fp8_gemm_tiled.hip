@@ -151,9 +151,6 @@ __global__ __launch_bounds__(WN * WT * KG * 64) void fp8_gemm_tiled_kernel(Fp8Ge
 #pragma unroll
             for (int j = 0; j < TF; ++j) xv[j][e] &= keep;
         }
-#pragma unroll
-        for (int j = 0; j < TF; ++j) xs_next[j] = kb < k_end ? xs_next[j] : 0.f;   // (no 0 x infinity behind the end)
-        ws_next = kb < k_end ? ws_next : 0.f;
     };
     auto scales = [&](int st) {
         const unsigned char *f = stages + (st % STAGES) * C::STAGE;
@@ -183,6 +180,11 @@ __global__ __launch_bounds__(WN * WT * KG * 64) void fp8_gemm_tiled_kernel(Fp8Ge
             if (k == 0) {
 #pragma unroll
                 for (int e = 0; e < TF; ++e) s[e] = xs_next[e] * ws_next;
+                if (KG > 1 && mode == LAST) {               // (no 0 x infinity where the second group has no block left)
+                    const bool has = block_of(st) < k_end;
+#pragma unroll
+                    for (int e = 0; e < TF; ++e) s[e] = has ? s[e] : 0.f;
+                }
             }
             p[k % DEPTH] = [&] {
                 const f32x4 prev = p[k % DEPTH];
