@@ -369,32 +369,34 @@ bool fp8_gemm_tiled_supported(const Fp8GemmArgs &a) {
 }
 
 // Tile shape and number of K ranges.  A launch lasts about  base + rounds * (round + steps * step)  us, rounds of 256 blocks
-// (a CU holds one), and longer per step when there are several rounds (the chip's clock and its caches are then shared by
-// work at full rate); K ranges make more blocks of fewer steps and cost a second launch and the partial sums' way through
-// memory; and no launch beats its weights' bytes.  Fitted to 75 shapes of 20 to 4096 tokens, 512 to 28672 features and 512 to
-// 14336 inputs, all tile shapes with 1 to 8 ranges each: 9 % rms from the measurements, the pick on average 1.5 % from
-// the best (worst 1.49x: 64 tokens, 6144 x 14336).
-struct TileShape { int bn, bt; double base, round, step, crowd; };
-constexpr TileShape TILE_SHAPES[] = {{256, 256, 0.3, 7.3, 1.27, 1.165}, {128, 128, 2.1, 3.2, 0.46, 1.13},
-                                     {128, 64, 2.5, 2.6, 0.316, 1.11}, {64, 64, 2.4, 2.2, 0.183, 1.12}};
+// (a CU holds one).  A step of the only round is longer the more blocks fetch weights of their own (load: the memory's latency
+// under load is what a block waits for), one of several rounds by `crowd` (clock and caches are shared by work at full rate).
+// K ranges make more blocks of fewer steps and cost a second launch and the partial sums' way through memory; and no
+// launch beats its weights' bytes.  Fitted to 468 shapes of 20 to 4096 tokens, 512 to 28672 features and 512 to 14336 inputs
+// with weights that come from HBM, all tile shapes with 1 to 8 ranges each: 9 % rms from the measurements, the pick on
+// average 0.7 % from the best (95 % of the shapes within 4 %, worst 1.29x: 20 tokens, 6144 x 8192).
+struct TileShape { int bn, bt; double base, round, step, crowd, load; };
+constexpr TileShape TILE_SHAPES[] = {{256, 256, 0.0, 7.0, 1.29, 1.21, 0.21}, {128, 128, 1.5, 3.1, 0.49, 1.18, 0.61},
+                                     {128, 64, 1.7, 2.8, 0.343, 1.11, 1.15}, {64, 64, 1.5, 2.45, 0.21, 1.12, 0.93}};
 constexpr size_t MAX_PART_BYTES = (size_t)64 << 20;
 
 static Fp8Plan tiled_plan(int T, int N, int K, size_t tmp_bytes) {
     const int kb = (K + FP8_GROUP - 1) / FP8_GROUP;
-    const double np = (N + 3) / 4 * 4.0, weights_us = (double)N * K / 4.5e6 + 3.0;
+    const double np = (N + 3) / 4 * 4.0, weights_us = (double)N * K / 5.2e6 + 4.5;
     Fp8Plan best{0, 1, 0};
     double best_us = 1e30;
     for (int i = 0; i < 4; ++i) {
         const TileShape &s = TILE_SHAPES[i];
-        const double tiles = (double)((N + s.bn - 1) / s.bn) * ((T + s.bt - 1) / s.bt);
+        const double tiles_t = (T + s.bt - 1) / s.bt, tiles = (double)((N + s.bn - 1) / s.bn) * tiles_t;
         for (int split = 1; split <= 8; split *= 2) {
             const int steps = (kb + split - 1) / split, ranges = (kb + steps - 1) / steps;
             const double part = ranges > 1 ? ranges * (double)T * np * 4 : 0;
             if (ranges > 1 && (steps < 4 || tiles * ranges > 600 || part > (double)tmp_bytes)) break;
             const double rounds = ceil(tiles * ranges / 256);
-            double us = s.base + rounds * (s.round + steps * s.step * (rounds > 1 ? s.crowd : 1.0));
+            const double slower = rounds > 1 ? s.crowd : 1 + s.load * tiles * ranges / 256 / tiles_t;
+            double us = s.base + rounds * (s.round + steps * s.step * slower);
             if (us < weights_us) us = weights_us;
-            if (ranges > 1) us += 2.7 + 2 * part / 3.7e6;
+            if (ranges > 1) us += 2.9 + 2 * part / 4.6e6;
             if (us < best_us) {
                 best_us = us;
                 best = Fp8Plan{i, ranges, (size_t)part};
