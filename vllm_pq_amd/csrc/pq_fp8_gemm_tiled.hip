@@ -10,6 +10,12 @@
 // one cycle ({0-3, 12-15, 20-27} and the like: rows 0-3 and 12-15 at piece c, rows 4-11 at piece c ^ 1) fall on 16
 // different groups of banks.  The DMA writes 64 lanes x 16 bytes in lane order, so it is the lanes' GLOBAL addresses that are
 // permuted; the 8 lanes of a row still read one 128-byte line.
+//
+// Measured: 4096 tokens of 28672 x 4096 411 to 440 us over several devices (2.2 to 2.35 PFLOP/s).  Of that the matrix
+// instructions alone take 268 us, with the LDS reads 296, with the sums 325; the rest is DMA and stores in the way of
+// both, at 1.9 GHz, which is what the power limit leaves of the clock.  512 tokens of 4096 x 4096 14.2 to 15.8 us (5 us of
+// it to start and end one round), 128 tokens of 4096 x 14336 18.4 us and 4 for adding the two ranges (a block has 48 KiB of
+// weights under way, and memory answers in 1.9 us).
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <math.h>
