@@ -316,6 +316,14 @@ def test_gpu_block_gemm_and_linear(T, N, K, dt):
 
 
 @gpu
+@pytest.mark.parametrize("T,N,K", [(3, 70, 2064), (4, 20, 1168), (2, 40, 2576), (1, 9000, 2048), (1, 33, 3600), (16, 600, 2176), (7, 8300, 2400),
+                                   (13, 24, 1151)])
+def test_gpu_few_tokens_any_number_of_blocks(T, N, K):
+    """9 to 29 scale blocks over 8 waves: two, three and four of a wave, whole and short, quantised inside and before."""
+    test_gpu_block_gemm_and_linear(T, N, K, "bf16")
+
+
+@gpu
 @pytest.mark.parametrize("T,N,K", [(2500, 6100, 1000), (2560, 6144, 1040), (1000, 4000, 1084), (1024, 4096, 512), (520, 4096, 2000),
                                    (250, 4096, 1152), (64, 512, 8192), (40, 1000, 14300), (300, 4096, 14336), (17, 257, 4100),
                                    (4096, 300, 260)])

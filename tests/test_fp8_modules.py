@@ -40,6 +40,15 @@ def test_config_key_and_method_choice():
         is_fp8_module("a.self_attn.qkv_proj", ["v_proj"])
 
 
+def test_one_expression_in_place_of_a_list_is_refused():
+    from vllm_pq_amd.quantize import quantization_config, quantize_state_dict
+    for call in (lambda: PQConfig(fp8_modules="down_proj"), lambda: quantization_config(8, 8, 1, "down_proj"),
+                 lambda: PQConfig.from_config({"in_group_size": 8, "nbits_per_codebook": 8, "fp8_modules": "down_proj"}),
+                 lambda: quantize_state_dict({}, fp8_modules="down_proj")):
+        with pytest.raises(ValueError, match="list of regular expressions"):
+            call()
+
+
 def test_create_weights_shapes_and_refusals(monkeypatch):
     cfg = PQConfig(fp8_modules=["."])
     layer = RowParallelLinear(300, 200, bias=False, params_dtype=BF16, quant_config=cfg, prefix="x")

@@ -58,6 +58,8 @@ class PQConfig(QuantizationConfig):
         super().__init__()
         # Regular expressions of the linear modules that the checkpoint holds as block-scaled e4m3 values instead (key of
         # the same name in the HF quantization_config); see fp8.py.
+        if isinstance(fp8_modules, str):
+            raise ValueError(f"fp8_modules must be a list of regular expressions, got {fp8_modules!r}")
         self.fp8_modules = list(fp8_modules or [])
         # After the load-time re-layout the kernels read only the packed copy of a linear layer's codes; with this
         # key (same name in the HF quantization_config) the reference-layout tensor gives its storage back (shape and

@@ -141,6 +141,8 @@ def quantization_config(d: int, nbits: int, num_codebooks: int = 1, fp8_modules:
     """The `quantization_config` entry of the HF config.json that selects this method (PQConfig.from_config)."""
     cfg: Dict[str, object] = {"quant_method": "pq", "in_group_size": d, "nbits_per_codebook": nbits,
                               "num_codebooks": num_codebooks, "out_group_size": 1}
+    if isinstance(fp8_modules, str):
+        raise ValueError(f"fp8_modules must be a list of regular expressions, got {fp8_modules!r}")
     if fp8_modules:
         cfg["fp8_modules"] = list(fp8_modules)
     return cfg
@@ -155,6 +157,8 @@ def quantize_state_dict(state: Dict[str, torch.Tensor], include: str = r".*(q_pr
     (the checkpoint names the reference's model loaders expect, vllm/model_executor/models/llama.py:371-433);
     other tensors pass through.  Modules that one of the `fp8_modules` expressions is found in become
     `<module>.weight` (e4m3) / `.weight_scale_inv` instead.  `report` collects (name, relative Frobenius error)."""
+    if isinstance(fp8_modules, str):
+        raise ValueError(f"fp8_modules must be a list of regular expressions, got {fp8_modules!r}")
     pat = re.compile(include)
     out: Dict[str, torch.Tensor] = {}
     for i, (name, t) in enumerate(state.items()):
