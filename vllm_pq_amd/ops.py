@@ -23,6 +23,7 @@ _CODE_BYTES = {torch.int8: 1, torch.int16: 2}
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device   # (no lazy initialisation to check)
 
 
 def _stream_ptr(device) -> int:
@@ -789,7 +790,7 @@ def _fp8_outputs(input: torch.Tensor, T: int, H: int, dev):
 
 def _call_on(dev, fn, *args) -> None:
     """fn(*args, stream) on `dev`, with the current stream of that device; raises what the library reports."""
-    if dev.index == torch.cuda.current_device():
+    if dev.index == _current_device():
         rc = fn(*args, _stream_ptr(dev))
     else:
         with torch.cuda.device(dev):
@@ -853,7 +854,8 @@ def _fp8_weight(what: str, K: int, weight: torch.Tensor, weight_scales: torch.Te
     if bias is not None:
         if bias.numel() != N or bias.dtype is not dtype:
             raise ValueError(f"{what}: bias must hold one value of {dtype} per output row")
-        bias = bias.reshape(-1).contiguous()
+        if bias.dim() != 1 or not bias.is_contiguous():
+            bias = bias.reshape(-1).contiguous()
         bptr = bias.data_ptr()
     w0 = K
     if not weight.is_contiguous():
@@ -874,28 +876,26 @@ def _fp8_tmp_bytes(fn: str, T: int, N: int, K: int) -> int:
 def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
                    bias: Optional[torch.Tensor], out_dtype: torch.dtype) -> torch.Tensor:
     what = "fp8_block_gemm"
-    if not input.is_cuda or scales.device != input.device:
+    dev = input.device
+    if not input.is_cuda or scales.device != dev:
         _check_device(input, scales, weight, weight_scales, bias)
-    if input.dtype != FP8_DTYPE or input.dim() < 1:
-        raise ValueError(f"{what}: input of {FP8_DTYPE} expected, got {tuple(input.shape)} {input.dtype}")
+    shape = input.shape
+    if input.dtype is not FP8_DTYPE or not shape:
+        raise ValueError(f"{what}: input of {FP8_DTYPE} expected, got {tuple(shape)} {input.dtype}")
     code = _DTYPE.get(out_dtype)
     if code is None:
         raise ValueError(f"{what}: out_dtype {out_dtype}: fp16 and bf16 are supported")
-    dev = input.device
-    lead = input.shape[:-1]
-    K = input.shape[-1]
+    flat = len(shape) == 2
+    T, K = shape if flat else (shape[:-1].numel(), shape[-1])
     groups = (K + FP8_GROUP - 1) // FP8_GROUP
-    if scales.dtype != torch.float32 or scales.shape != lead + (groups,):
-        raise ValueError(f"{what}: scales {tuple(lead) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
+    if scales.dtype is not torch.float32 or scales.shape != ((T, groups) if flat else shape[:-1] + (groups,)):
+        raise ValueError(f"{what}: scales {tuple(shape[:-1]) + (groups,)} fp32 expected, got {tuple(scales.shape)} {scales.dtype}")
     weight, w0, N, weight_scales, bptr, bias = _fp8_weight(what, K, weight, weight_scales, bias, out_dtype, dev)
-    T = lead.numel()
     if T >> 31:
         raise ValueError(f"{what}: {T} tokens: sizes below 2^31 are supported")
     out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=dev)
-    if len(lead) != 1:
-        out = out.view(lead + (N,))
     if T and N:
-        q2, s2 = (input, scales) if len(lead) == 1 else (input.reshape(T, K), scales.reshape(T, groups))
+        q2, s2 = (input, scales) if flat else (input.reshape(T, K), scales.reshape(T, groups))
         q0, q1 = q2.stride()
         if (q1 != 1 and K > 1) or (q0 < K and T > 1):
             q2 = q2.contiguous()
@@ -906,7 +906,7 @@ def _fp8_gemm_impl(input: torch.Tensor, scales: torch.Tensor, weight: torch.Tens
         _call_on(dev, _lib.load().pq_fp8_block_gemm, q2.data_ptr(), T, q0 if T > 1 else K, s2.data_ptr(), st, sg,
                  weight.data_ptr(), w0, weight_scales.data_ptr(), groups, bptr, N, K, code, out.data_ptr(), N,
                  None if tmp is None else tmp.data_ptr(), nbytes)
-    return out
+    return out if flat else out.view(shape[:-1] + (N,))
 
 
 def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
