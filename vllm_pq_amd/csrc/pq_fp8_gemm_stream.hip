@@ -214,8 +214,10 @@ bool fp8_gemm_stream_supported(const Fp8GemmArgs &a) {
            (tmp == 0 || (a.tmp && a.tmp_bytes >= tmp));
 }
 
-// Every block quantises for itself, which beats a launch in front while it takes less than that: 1 token of 6144 x 4096
-// 9.9 us against 9.4 + 2.6, 2 tokens 10.4 against 8.9 + 2.7, 4 tokens 13.5 against 9.1 + 2.8.
+// Every block quantises for itself, which beats a launch in front while it takes less than that.  Inside against apart, in a
+// graph with weights from HBM: 1 token of 28672 x 4096 25.1 us against 27.3, 2 tokens 25.7 against 28.5, 8 of 4096 x 1024 5.4
+// against 6.0, 4 of 8192 x 2048 8.3 against 8.5, 2 of 6144 x 4096 11.9 against 11.7; with 16384 values (4 of 6144 x 4096) the
+// product alone grows from 9.1 to 13.5, more than the 2.8 of the launch.
 bool fp8_linear_fused(int T, int K) { return T <= 16 && K >= 16 && K % 16 == 0 && K <= SM_RANGE * FP8_GROUP && T * K <= SM_MAX_FUSED; }
 
 hipError_t launch_fp8_gemm_stream(const Fp8GemmArgs &a, hipStream_t stream) {
