@@ -168,6 +168,10 @@ def test_gemm_refusals_need_no_gpu(linear):
         assert _gemm_rc(st=-1) == 1 and _gemm_rc(s=None) == 1 and _gemm_rc(tmp=264) == 1
 
 
+def test_linear_refuses_rows_too_far_apart():
+    assert _gemm_rc(True, T=1, wst=2 ** 26) == 2 and "weight_row_stride" in _lib.last_error()     # where it quantises inside
+
+
 def test_ops_raise_on_cpu_tensors():
     x, w = torch.zeros(2, 256, dtype=torch.bfloat16), torch.zeros(128, 256).to(F8)
     ws, one = torch.ones(1, 2), torch.ones(256, dtype=torch.bfloat16)
@@ -636,3 +640,51 @@ def test_fake_implementations_match_the_real_layouts():
         w = torch.empty(70, 300, dtype=F8, device="cuda")
         y = torch.ops.pq_amd.fp8_block_gemm(q, s, w, torch.empty(1, 3, device="cuda"), None, torch.float16)
         assert y.shape == (3, 5, 70) and y.dtype == torch.float16
+
+
+@gpu
+@pytest.mark.parametrize("T,N,K", [(40, 512, 8192), (300, 200, 1001), (4, 300, 8200), (1, 512, 1024), (128, 256, 4096)])
+def test_gpu_scratch_in_graphs_and_on_two_streams(T, N, K):
+    """Calls that use scratch (ranges of K, laid-out operands): two graphs of them replayed in turn while weights and scales change,
+    and two streams at once."""
+    gen = torch.Generator().manual_seed(T * K)
+    dt = torch.bfloat16
+    sets = []
+    for _ in range(2):
+        x = activations(gen, T, K, dt).to(DEV)
+        w, ws = (t.to(DEV) for t in weight(gen, N, K))
+        sets.append((x, w, ws))
+
+    def call(x, w, ws):
+        return ops.fp8_block_gemm(*ops.fp8_group_quant(x), w, ws), ops.fp8_block_linear(x, w, ws)
+    for a in sets:
+        call(*a)
+    torch.cuda.synchronize()
+    graphs = []
+    for a in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call(*a)
+        graphs.append((g, out))
+    for i in range(3):
+        for x, w, ws in sets:
+            x.copy_(activations(gen, T, K, dt))
+            fresh, scales = weight(gen, N, K)
+            w.view(torch.uint8).copy_(fresh.view(torch.uint8))
+            ws.copy_(scales)
+        for g, _ in graphs:
+            g.replay()
+        want = [call(*a) for a in sets]
+        for (_, got), w in zip(graphs, want):
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        results = []
+        for s, a in zip(streams, sets):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                results.append([call(*a) for _ in range(4)])
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        for many, w in zip(results, want):
+            for got in many:
+                assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
