@@ -260,6 +260,29 @@ def test_gpu_quant_extremes():
 
 
 @gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_gpu_silu_extremes(dt):
+    """The type's lowest and largest values in either half (masked or unset rows), gates far below zero, products near the end
+    of fp32, infinities and NaN.  Where silu is not 0 the gates are within 16 of 0, so V holds as it does above."""
+    dt = DT[dt]
+    low, high = torch.finfo(dt).min, torch.finfo(dt).max
+    rows = [(low, low), (low, 1.0), (low, high), (-1000.0, high), (-1.0, low), (-5.0, low), (-0.0, low), (1.0, high / 2), (low, 0.0), (0.0, high),
+            (high / 4, 1.0), (-300.0, -2.0)]
+    g = torch.stack([torch.full((128,), a) for a, _ in rows]).to(dt)
+    u = torch.stack([torch.full((128,), b) for _, b in rows]).to(dt)
+    u[:, 64:] *= 0.5
+    q, s = (t.cpu() for t in ops.silu_and_mul_fp8(torch.cat((g, u), 1).to(DEV)))
+    v = g.double() * torch.sigmoid(g.double()) * u.double()
+    assert torch.isfinite(s).all()
+    check_quant(q, s, v, True)
+    for a, b in ((math.inf, 1.0), (-math.inf, 1.0), (math.nan, 1.0), (1.0, math.inf), (1.0, math.nan)):
+        g[0], u[0] = 1.0, 1.0
+        g[0, 5], u[0, 5] = a, b
+        s = ops.silu_and_mul_fp8(torch.cat((g, u), 1).to(DEV))[1].cpu()
+        assert not math.isfinite(s[0, 0]) and torch.isfinite(s[1:]).all()
+
+
+@gpu
 def test_gpu_quant_strides_shapes_and_empty():
     gen = torch.Generator().manual_seed(2)
     base = activations(gen, 12, 700, torch.bfloat16)

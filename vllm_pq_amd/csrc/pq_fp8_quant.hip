@@ -14,7 +14,7 @@
 // All are bound by HBM (2 bytes in, 1 out per value) or, for a few tokens, by the launch.  One thread owns 8 consecutive
 // values (one 16-byte load, at any alignment; the last piece of a row may be shorter), 16 neighbouring lanes a group: its
 // maximum is four lane exchanges, nothing passes through LDS.  Measured: 4096 x 14336 bf16 32.3 us (5.4 TB/s of the bytes named
-// above; a plain copy reaches 5.0), silu_and_mul 51 to 54 us (5.5 TB/s), the norm with a residual of 4096 x 8192 fp16 42.3 us
+// above; a plain copy reaches 5.0), silu_and_mul 55 us (5.3 TB/s), the norm with a residual of 4096 x 8192 fp16 42.3 us
 // (5.6 TB/s); 16 rows of 4096 2.6 to 3.4 us, which is what an empty launch takes.
 #include <hip/hip_runtime.h>
 
@@ -35,14 +35,18 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
     return umax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
 }
 
-// silu(g) * u in fp32, about a unit of the last place off.  exp(-g) as 2^t, t = -g log2(e): what t's rounding leaves out (up
-// to |t| 2^-24 of the result) is put back to first order; the reciprocal gets one Newton step.  Below -87 the exponential
-// stands still (silu is under 2^-118 there), so no infinity comes up that g does not bring.
+// silu(g) * u = g u / (1 + exp(-g)) in fp32.  The product of two act-dtype values is exact in fp32 and the quotient correctly
+// rounded (one Newton step on its residual), so the error is that of the exponential: 2^t, t = -g log2(e), where what t's
+// rounding leaves out (up to |t| 2^-24 of the result) is put back to first order.  Numerator and denominator carry a factor of
+// 2^-8, so that g u stays finite wherever the result does.  Below -88 g counts as 0 (silu is under 2^-120 there): the type's
+// lowest value gives nothing.  An infinity in g comes through u, as NaN.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-    constexpr float L = 1.4426950408889634f, L_LO = (float)(1.4426950408889634074 - (double)L), LN2 = 0.6931471805599453f;
-    const float x = fmaxf(g, -87.0f), t = -x * L, rest = __builtin_fmaf(-x, L_LO, __builtin_fmaf(-x, L, -t));
-    const float p = __builtin_amdgcn_exp2f(t), d = 1.0f + __builtin_fmaf(p * rest, LN2, p), r = __builtin_amdgcn_rcpf(d);
-    return g * __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) * u;
+    constexpr float L = 1.4426950408889634f * 256, L_LO = (float)(1.4426950408889634074 * 256 - (double)L), LN2 = 0.6931471805599453f;
+    constexpr float S = 0x1p-8f;
+    const float x = g < -88.0f ? 0.0f : g * S, t = -x * L, rest = __builtin_fmaf(-x, L_LO, __builtin_fmaf(-x, L, -t));
+    const float e = __builtin_amdgcn_exp2f(t), d = (1.0f + __builtin_fmaf(e * rest, LN2, e)) * S, r = __builtin_amdgcn_rcpf(d);
+    const float p = x * __builtin_fmaf(g, 0.0f, u), q = p * r;
+    return __builtin_fmaf(__builtin_fmaf(-d, q, p), r, q);
 }
 
 // 8 act-dtype values from any address; WHOLE: all of a row's pieces have 8, else the first `valid` and zeros behind, nothing
