@@ -226,6 +226,35 @@ def test_gpu_norm_fp8(T, H, add, dt):
 
 
 @gpu
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("eps", [1e-5, 1e-30])
+def test_gpu_norm_fp8_small_values(eps, add):
+    """Rows and groups far below 1: the floor 2^-96 is one of the normed values, which 1 / rms makes up to 316 (1e15) times as
+    large.  The values are known to V there too: z is exact, z^2 and its sum count only where they are beside eps, and a
+    subnormal step (2^-149) is below V of the smallest numbers that matter (2^-10 of 2^-96 / 448, over rms)."""
+    gen = torch.Generator().manual_seed(5)
+    H, dt = 640, torch.bfloat16
+    size = torch.zeros(9, H)
+    for row, exponent in enumerate((-90, -97, -100, -104, -110), 1):
+        size[row] = 2.0 ** exponent
+    size[6], size[6, 128:256] = 2.0 ** -5, 2.0 ** -99          # small groups beside ordinary ones
+    size[7], size[7, :128] = 2.0 ** -40, 2.0 ** -110
+    size[8], size[8, 256:384] = 1.0, 2.0 ** -96
+    x, res = ((torch.randn(9, H, generator=gen) * size).to(dt) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(H, generator=gen)).to(dt)
+    z = x.float() + res.float() if add else x.float()
+    if add:
+        rd = res.to(DEV)
+        q, s = ops.fused_add_rms_norm_fp8(x.to(DEV), rd, w.to(DEV), eps)
+        assert torch.equal(rd.cpu(), z.to(dt))
+    else:
+        q, s = ops.rms_norm_fp8(x.to(DEV), w.to(DEV), eps)
+    z = z.double()
+    check_quant(q, s, z / torch.sqrt((z * z).mean(-1, keepdim=True) + eps) * w.double(), True)
+    assert not q[0].float().any() and (s[0].cpu() == torch.tensor(2.0 ** -96) / 448).all()
+
+
+@gpu
 def test_gpu_quant_extremes():
     """Zeros, a single value, the largest and smallest values, ties between two e4m3 numbers, infinities and NaN."""
     x = torch.zeros(10, 256, dtype=torch.bfloat16)

@@ -127,9 +127,11 @@ __global__ __launch_bounds__(QT) void quant_kernel(QuantArgs a) {
 // ---- with a norm -----------------------------------------------------------------------------------------
 // One block of THREADS per token row; the row stays in registers between the sum of squares and the scaling, as in
 // rms_norm_kernel.  ADD: z = x + residual, the residual becomes the rounded sum (the norm uses the unrounded one).
-// 1 / rms is a factor of a group's values and of its scale alike, so the quotients are taken without it,
-//   q = e4m3(u / (max |u| / 448)),  s = max |u| / 448 / rms,  u = z w:
-// one rounding and one product less per value.
+// 1 / rms = 2^e f, f in [1, 2), is a factor of a group's values and of its scale alike, so the quotients are taken with its
+// power of two alone, which rounds nothing,
+//   q = e4m3(u / (max |u| / 448)),  s = max |u| / 448 f,  u = 2^e z w:
+// one rounding less per value.  The floor 2^-96 holds for max |u| f, the normed values, and becomes 2^-96 / f in the quotients;
+// 2^e keeps u within a factor of 2 of them, so that a row of small values leaves no quotient of subnormal numbers.
 template <typename AT, int THREADS, int NV, bool ADD, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void norm_quant_kernel(QuantArgs a) {
     __shared__ float s_part[THREADS / 64];
@@ -166,6 +168,9 @@ __global__ __launch_bounds__(THREADS) void norm_quant_kernel(QuantArgs a) {
         }
     }
     const float rs = rsqrtf(block_sum<THREADS>(ss, s_part) / (float)a.H + a.eps);
+    const bool plain = __builtin_isnormal(rs);     // 0, infinite or NaN: the values take it as it is
+    const float pow2 = plain ? __uint_as_float(__float_as_uint(rs) & 0x7f800000u) : rs;
+    const float frac = plain ? __uint_as_float((__float_as_uint(rs) & 0x007fffffu) | 0x3f800000u) : 1.f;
     uint8_t *qr = static_cast<uint8_t *>(a.q) + t * a.q_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -174,16 +179,14 @@ __global__ __launch_bounds__(THREADS) void norm_quant_kernel(QuantArgs a) {
             float w[8];
             unpack8<AT>(raw8<WHOLE, false>(static_cast<const uint16_t *>(a.weight) + v * 8, valid), w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) z[i][j] *= w[j];
+            for (int j = 0; j < 8; ++j) z[i][j] = z[i][j] * pow2 * w[j];
         }
-        const uint32_t m = group_max(amax8(z[i]));
-        const float amax = __uint_as_float(m) * rs;               // of the normed values
-        const bool low = amax < __uint_as_float(AMAX_MIN_BITS);   // (a NaN is not low)
-        const GroupScale g = low ? group_scale(abs_bits(__uint_as_float(AMAX_MIN_BITS) / rs)) : group_scale(m);
+        const float floor = __uint_as_float(AMAX_MIN_BITS), m = __uint_as_float(group_max(amax8(z[i]))), amax = m * frac;
+        const bool low = amax < floor;                            // (a NaN is not low)
+        const GroupScale g = scale_of(low ? floor / frac : m);
         if (valid > 0) {
             store8<WHOLE>(qr + v * 8, valid, z[i], g);
-            if (threadIdx.x % QV == 0)
-                a.scales[(int64_t)(v / QV) * a.scale_stride + t] = low ? __uint_as_float(AMAX_MIN_BITS) / FP8_MAX : amax / FP8_MAX;
+            if (threadIdx.x % QV == 0) a.scales[(int64_t)(v / QV) * a.scale_stride + t] = (low ? floor : amax) / FP8_MAX;
         }
     }
 }

@@ -13,12 +13,15 @@ constexpr uint32_t AMAX_MIN_BITS = (127 - 96) << 23;   // 2^-96
 struct GroupScale {
     float s, r, c;
 };
-__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
+__device__ __forceinline__ GroupScale scale_of(float amax) {      // no floor: amax far enough from 0 that amax / 448 is normal
     GroupScale g;
-    g.s = __uint_as_float(amax_bits > AMAX_MIN_BITS ? amax_bits : AMAX_MIN_BITS) / FP8_MAX;
+    g.s = amax / FP8_MAX;
     g.r = __builtin_amdgcn_rcpf(g.s);         // within one unit of the last place
     g.c = __builtin_isinf(g.s) ? 0.f : g.s;   // an infinite scale: v * r stands as it is (0, or NaN for the infinity itself)
     return g;
+}
+__device__ __forceinline__ GroupScale group_scale(uint32_t amax_bits) {
+    return scale_of(__uint_as_float(amax_bits > AMAX_MIN_BITS ? amax_bits : AMAX_MIN_BITS));
 }
 // v / s in fp32: the product with the reciprocal is within 2^-22 of the quotient, and one Newton step on its exact residual
 // takes that to 2^-44, so the rounded result is the correctly rounded quotient unless that lies within 2^-44 of half way
