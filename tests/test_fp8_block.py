@@ -312,6 +312,22 @@ def test_gpu_silu_extremes(dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_gpu_silu_largest_gates(dt):
+    """Gates up to the type's largest value, each product finite in fp32.  Above 88 silu(g) is g to the last place."""
+    dt = DT[dt]
+    high = torch.finfo(dt).max
+    gates = [88.5, 127.0, 128.0, 129.0, 200.0, 1000.0, high / 4, high / 2, 0.7 * high, 0.75 * high, high]
+    g = torch.tensor([[a] * 128 for a in gates for _ in range(4)]).to(dt)
+    u = torch.tensor([[0.5, 1.0, -0.25, 0.0]] * len(gates)).view(-1, 1).repeat(1, 128).to(dt)
+    u[:, 64:] *= 0.5
+    g[:, 1::2] = torch.linspace(-15.0, 88.0, 64).to(dt)       # beside ordinary ones
+    q, s = (t.cpu() for t in ops.silu_and_mul_fp8(torch.cat((g, u), 1).to(DEV)))
+    assert torch.isfinite(s).all() and torch.isfinite(q.float()).all()
+    check_quant(q, s, g.double() * torch.sigmoid(g.double()) * u.double(), True)
+
+
+@gpu
 def test_gpu_quant_strides_shapes_and_empty():
     gen = torch.Generator().manual_seed(2)
     base = activations(gen, 12, 700, torch.bfloat16)

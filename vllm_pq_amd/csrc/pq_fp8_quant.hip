@@ -38,12 +38,14 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 // silu(g) * u = g u / (1 + exp(-g)) in fp32.  The product of two act-dtype values is exact in fp32 and the quotient correctly
 // rounded (one Newton step on its residual), so the error is that of the exponential: 2^t, t = -g log2(e), where what t's
 // rounding leaves out (up to |t| 2^-24 of the result) is put back to first order.  Numerator and denominator carry a factor of
-// 2^-8, so that g u stays finite wherever the result does.  Below -88 g counts as 0 (silu is under 2^-120 there): the type's
-// lowest value gives nothing.  An infinity in g comes through u, as NaN.
+// 2^-8, so that g u stays finite wherever the result does.  The exponential takes g as at most 128, where it is far below
+// 1's last place, so that t stays finite at the type's largest value.  Below -88 g counts as 0 (silu is under 2^-120 there):
+// the type's lowest value gives nothing.  An infinity in g comes through u, as NaN, and so does a NaN.
 __device__ __forceinline__ float silu_mul(float g, float u) {
     constexpr float L = 1.4426950408889634f * 256, L_LO = (float)(1.4426950408889634074 * 256 - (double)L), LN2 = 0.6931471805599453f;
     constexpr float S = 0x1p-8f;
-    const float x = g < -88.0f ? 0.0f : g * S, t = -x * L, rest = __builtin_fmaf(-x, L_LO, __builtin_fmaf(-x, L, -t));
+    const float x = g < -88.0f ? 0.0f : g * S;
+    const float y = fminf(x, 128.0f * S), t = -y * L, rest = __builtin_fmaf(-y, L_LO, __builtin_fmaf(-y, L, -t));
     const float e = __builtin_amdgcn_exp2f(t), d = (1.0f + __builtin_fmaf(e * rest, LN2, e)) * S, r = __builtin_amdgcn_rcpf(d);
     const float p = x * __builtin_fmaf(g, 0.0f, u), q = p * r;
     return __builtin_fmaf(__builtin_fmaf(-d, q, p), r, q);
