@@ -328,6 +328,29 @@ def test_gpu_silu_largest_gates(dt):
 
 
 @gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_gpu_silu_gates_far_below_zero(dt):
+    """silu(-90) is 1e-37, which a large u makes an ordinary number again.  The exponential's error grows with the rounded
+    exponent put back to first order only, (|t| 2^-24)^2: below V by far."""
+    dt = DT[dt]
+    high = torch.finfo(dt).max
+    gates = [-80.0, -87.0, -87.5, -88.0, -88.5, -90.0, -100.0, -104.0, -125.0, -150.0, -170.0, -174.0, -175.0, -176.0, -200.0]
+    g = torch.tensor([[a] * 128 for a in gates for _ in range(4)]).to(dt)
+    u = torch.tensor([[high, -high / 2, 1.0, -high / 64]] * len(gates)).view(-1, 1).repeat(1, 128).to(dt)
+    u[:, 1::2] *= 0.625
+    g[:, 64:] += 1.0 / 2
+    near = (2 * torch.randn(len(g), 256, generator=torch.Generator().manual_seed(1))).to(dt)
+    gg, uu = torch.cat((g, near), 1), torch.cat((u, near.flip(1)), 1)         # two ordinary groups beside each
+    q, s = (t.cpu() for t in ops.silu_and_mul_fp8(torch.cat((gg, uu), 1).to(DEV)))
+    assert torch.isfinite(s).all()
+    check_quant(q, s, gg.double() * torch.sigmoid(gg.double()) * uu.double(), True)
+    # and those keep their bits where the gates beside them are ordinary too
+    gg[:, :128] = 1.0
+    q1, s1 = (t.cpu() for t in ops.silu_and_mul_fp8(torch.cat((gg, uu), 1).to(DEV)))
+    assert torch.equal(q1[:, 128:].float(), q[:, 128:].float()) and torch.equal(s1[:, 1:], s[:, 1:])
+
+
+@gpu
 def test_gpu_quant_strides_shapes_and_empty():
     gen = torch.Generator().manual_seed(2)
     base = activations(gen, 12, 700, torch.bfloat16)

@@ -14,7 +14,7 @@
 // All are bound by HBM (2 bytes in, 1 out per value) or, for a few tokens, by the launch.  One thread owns 8 consecutive
 // values (one 16-byte load, at any alignment; the last piece of a row may be shorter), 16 neighbouring lanes a group: its
 // maximum is four lane exchanges, nothing passes through LDS.  Measured: 4096 x 14336 bf16 32.3 us (5.4 TB/s of the bytes named
-// above; a plain copy reaches 5.0), silu_and_mul 55 us (5.3 TB/s), the norm with a residual of 4096 x 8192 fp16 42.3 us
+// above; a plain copy reaches 5.0), silu_and_mul 52 us (5.6 TB/s), the norm with a residual of 4096 x 8192 fp16 42.3 us
 // (5.6 TB/s); 16 rows of 4096 2.6 to 3.4 us, which is what an empty launch takes.
 #include <hip/hip_runtime.h>
 
@@ -38,17 +38,40 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 // silu(g) * u = g u / (1 + exp(-g)) in fp32.  The product of two act-dtype values is exact in fp32 and the quotient correctly
 // rounded (one Newton step on its residual), so the error is that of the exponential: 2^t, t = -g log2(e), where what t's
 // rounding leaves out (up to |t| 2^-24 of the result) is put back to first order.  Numerator and denominator carry a factor of
-// 2^-8, so that g u stays finite wherever the result does.  The exponential takes g as at most 128, where it is far below
-// 1's last place, so that t stays finite at the type's largest value.  Below -88 g counts as 0 (silu is under 2^-120 there):
-// the type's lowest value gives nothing.  An infinity in g comes through u, as NaN, and so does a NaN.
+// 2^-8, so that g u stays finite wherever the result does.  A NaN in g comes through.
+//
+// FAR is for gates beyond 88 on either side, of which there are none in most waves:
+//   - the exponential takes g as at most 128, where it is far below 1's last place, so that t stays finite at the type's
+//     largest value;
+//   - below -87.5 numerator and denominator carry 2^-125 more, which 2^t alone would not hold;
+//   - below -174 g counts as 0: |silu(g) u| < 2^-115 for every finite u, less than half of the smallest value that e4m3 holds
+//     beside the floor's scale (2^-9 * 2^-96 / 448), so the type's lowest value gives nothing;
+//   - an infinity in g comes through u, as NaN.
+// For the other gates it computes the same bits.
+template <bool FAR>
 __device__ __forceinline__ float silu_mul(float g, float u) {
     constexpr float L = 1.4426950408889634f * 256, L_LO = (float)(1.4426950408889634074 * 256 - (double)L), LN2 = 0.6931471805599453f;
     constexpr float S = 0x1p-8f;
-    const float x = g < -88.0f ? 0.0f : g * S;
-    const float y = fminf(x, 128.0f * S), t = -y * L, rest = __builtin_fmaf(-y, L_LO, __builtin_fmaf(-y, L, -t));
-    const float e = __builtin_amdgcn_exp2f(t), d = (1.0f + __builtin_fmaf(e * rest, LN2, e)) * S, r = __builtin_amdgcn_rcpf(d);
-    const float p = x * __builtin_fmaf(g, 0.0f, u), q = p * r;
+    const float x = FAR && g < -174.0f ? 0.0f : g * S, y = FAR && x > 128.0f * S ? 128.0f * S : x;
+    const bool low = FAR && x < -87.5f * S;
+    const float one = low ? 0x1p-125f : 1.0f, t = -y * L, rest = __builtin_fmaf(-y, L_LO, __builtin_fmaf(-y, L, -t));
+    const float e = __builtin_amdgcn_exp2f(low ? t - 125.0f : t);
+    const float d = (one + __builtin_fmaf(e * rest, LN2, e)) * S, r = __builtin_amdgcn_rcpf(d);
+    const float p = FAR ? x * __builtin_fmaf(g, 0.0f, u) * one : x * u, q = p * r;
     return __builtin_fmaf(__builtin_fmaf(-d, q, p), r, q);
+}
+// f = silu(f) * u for 8 values
+__device__ __forceinline__ void silu_mul8(float *f, const float *u) {
+    float far = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) far = fmaxf(far, __builtin_fabsf(f[j]));
+    if (__builtin_amdgcn_ballot_w64(far > 87.5f)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = silu_mul<true>(f[j], u[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = silu_mul<false>(f[j], u[j]);
+    }
 }
 
 // 8 act-dtype values from any address; WHOLE: all of a row's pieces have 8, else the first `valid` and zeros behind, nothing
@@ -115,8 +138,7 @@ __global__ __launch_bounds__(QT) void quant_kernel(QuantArgs a) {
         if constexpr (SILU) {
             float u[8];
             unpack8<AT>(second[i], u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = silu_mul(f[j], u[j]);
+            silu_mul8(f, u);
         }
         const GroupScale g = group_scale(group_max(valid > 0 ? amax8(f) : 0u));
         if (valid > 0 && t < a.T) {
