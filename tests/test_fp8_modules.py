@@ -133,6 +133,48 @@ def test_quantise_command_writes_both_formats(tmp_path, capsys):
     assert cfg.fp8_modules == ["down_proj"]
 
 
+def _attention_state(head="model.layers.0."):
+    names = [f"{head}self_attn.{n}_proj" for n in "qkvo"] + [f"{head}mlp.{n}_proj" for n in ("gate", "up", "down")]
+    return {n + ".weight": _dense(i, 128, 128) for i, n in enumerate(names)}
+
+
+@pytest.mark.parametrize("fp8", [["qkv_proj"], ["gate_up_proj"], ["gate_up"], ["self_attn"], ["[qkv]_proj"], ["o_proj", "qkv_proj$"], [r"\.0\.mlp"],
+                                 ["."], ["q_proj", "k_proj", "v_proj", "down_proj"]])
+def test_quantiser_and_loader_choose_alike(fp8):
+    """Whatever the expressions, a layer that the config makes an e4m3 one finds e4m3 tensors, and the others find codes."""
+    from vllm_pq_amd.quantize import quantization_config, quantize_state_dict
+    state = _attention_state()
+    out = quantize_state_dict(state, iters=1, fp8_modules=fp8)
+    cfg = PQConfig.from_config(quantization_config(8, 8, 1, fp8))
+    kinds = set()
+    for layer, parts in (("self_attn.qkv_proj", ("q_proj", "k_proj", "v_proj")), ("self_attn.o_proj", ("o_proj",)),
+                         ("mlp.gate_up_proj", ("gate_proj", "up_proj")), ("mlp.down_proj", ("down_proj",))):
+        prefix = "model.layers.0." + layer
+        method = type(ColumnParallelLinear(128, 128, bias=False, params_dtype=BF16, quant_config=cfg, prefix=prefix).quant_method)
+        kinds.add(method)
+        for n in parts:
+            base = prefix.rpartition(".")[0] + "." + n
+            has = {k for k in ("weight", "weight_scale_inv", "codes", "codebooks", "scales") if f"{base}.{k}" in out}
+            assert has == ({"weight", "weight_scale_inv"} if method is BlockFP8LinearMethod else {"codes", "codebooks", "scales"})
+    assert BlockFP8LinearMethod in kinds
+
+
+def test_quantiser_refuses_what_the_loader_would():
+    from vllm_pq_amd.quantize import quantize_state_dict
+    state = _attention_state()
+    for fp8 in (["v_proj"], ["up_proj"], ["down_proj", "gate_proj"], ["q_proj", "k_proj"]):
+        with pytest.raises(ValueError, match="only a part"):
+            quantize_state_dict(state, iters=1, fp8_modules=fp8)
+    # a q_proj that nothing is stacked with goes by its own name, as the layer of that name does
+    alone = {"m.q_proj.weight": state["model.layers.0.self_attn.q_proj.weight"]}
+    assert "m.q_proj.weight_scale_inv" in quantize_state_dict(alone, fp8_modules=["q_proj"])
+    # and a matrix that is stacked on disk already by the stacked layer's
+    stacked = {"m.qkv_proj.weight": _dense(0, 384, 128)}
+    assert "m.qkv_proj.weight_scale_inv" in quantize_state_dict(stacked, fp8_modules=["qkv_proj"])
+    with pytest.raises(ValueError, match="only a part"):
+        quantize_state_dict(stacked, fp8_modules=["v_proj"])
+
+
 def test_method_raises_on_cpu():
     layer = ColumnParallelLinear(256, 128, bias=False, params_dtype=BF16, quant_config=PQConfig(fp8_modules=["."]), prefix="x")
     m, x = layer.quant_method, torch.zeros(2, 256, dtype=BF16)

@@ -10,7 +10,7 @@ Activations are quantised per token and group of 128 features when the layer run
 the step in front of the layer (apply_after_norm, apply_after_silu_and_mul).
 """
 import re
-from typing import List, Optional, Tuple
+from typing import Iterable, List, Optional, Set, Tuple
 
 import torch
 from torch.nn.parameter import Parameter
@@ -31,6 +31,23 @@ def is_fp8_module(prefix: str, patterns: List[str]) -> bool:
     if found and found != names:
         raise ValueError(f"fp8_modules names only a part of what {prefix} stacks: {', '.join(found)}")
     return bool(found) or any(re.search(p, prefix) for p in patterns)
+
+
+def checkpoint_fp8_modules(modules: Iterable[str], patterns: List[str]) -> Set[str]:
+    """Those of a checkpoint's modules that become e4m3 layers under `patterns`: a module goes by the layer that stacks it where
+    the checkpoint holds all that this layer stacks, else by its own name, and either by is_fp8_module, as a model that loads
+    the checkpoint has it."""
+    modules = set(modules)
+    found = set()
+    for m in modules:
+        head, _, last = m.rpartition(".")
+        layer = m
+        for fused, parts in _FUSED.items():
+            if last in parts and all((f"{head}.{n}" if head else n) in modules for n in parts):
+                layer = f"{head}.{fused}" if head else fused
+        if is_fp8_module(layer, patterns):
+            found.add(m)
+    return found
 
 
 def fp8_quantize_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

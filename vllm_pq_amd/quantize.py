@@ -27,7 +27,7 @@ from typing import Dict, Iterable, List, Optional, Tuple
 
 import torch
 
-from .fp8 import fp8_quantize_weight, fp8_reconstruct
+from .fp8 import checkpoint_fp8_modules, fp8_quantize_weight, fp8_reconstruct
 from .pq import get_int_dtype
 
 __all__ = ["pq_quantize_weight", "pq_reconstruct", "quantize_state_dict", "save_pq_checkpoint", "quantization_config"]
@@ -155,15 +155,18 @@ def quantize_state_dict(state: Dict[str, torch.Tensor], include: str = r".*(q_pr
                         fp8_modules: Optional[List[str]] = None) -> Dict[str, torch.Tensor]:
     """Replace every `<module>.weight` whose name matches `include` by `<module>.codes/.codebooks/.scales`
     (the checkpoint names the reference's model loaders expect, vllm/model_executor/models/llama.py:371-433);
-    other tensors pass through.  Modules that one of the `fp8_modules` expressions is found in become
-    `<module>.weight` (e4m3) / `.weight_scale_inv` instead.  `report` collects (name, relative Frobenius error)."""
+    other tensors pass through.  Modules that the `fp8_modules` expressions name, by the rule the loader goes by (PQConfig: a
+    fused layer's parts all or none, by their names or the layer's), become `<module>.weight` (e4m3) / `.weight_scale_inv`
+    instead; `state` then holds whole layers.  `report` collects (name, relative Frobenius error)."""
     if isinstance(fp8_modules, str):
         raise ValueError(f"fp8_modules must be a list of regular expressions, got {fp8_modules!r}")
     pat = re.compile(include)
+    fp8 = checkpoint_fp8_modules([n[:-len(".weight")] for n, t in state.items() if t.dim() == 2 and pat.match(n)],
+                                 fp8_modules) if fp8_modules else ()
     out: Dict[str, torch.Tensor] = {}
     for i, (name, t) in enumerate(state.items()):
         base = name[:-len(".weight")]
-        if t.dim() == 2 and pat.match(name) and any(re.search(p, base) for p in fp8_modules or ()):
+        if t.dim() == 2 and pat.match(name) and base in fp8:
             w = t.to(device) if device else t
             q, scale = fp8_quantize_weight(w)
             if report is not None:
@@ -205,7 +208,8 @@ def _main(argv: Optional[Iterable[str]] = None) -> int:
     ap.add_argument("--num-codebooks", type=int, default=1)
     ap.add_argument("--iters", type=int, default=25)
     ap.add_argument("--fp8", action="append", default=[], metavar="REGEX",
-                    help="keep modules whose name contains this expression in block-scaled e4m3 (may be given again)")
+                    help="keep modules whose name, or the name of the fused layer they are stacked in, contains this expression in "
+                         "block-scaled e4m3 (may be given again; of a fused layer all parts or none)")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     args = ap.parse_args(argv)
     files = [args.input] if args.input.endswith(".safetensors") else \
