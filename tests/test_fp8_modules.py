@@ -175,6 +175,18 @@ def test_quantiser_refuses_what_the_loader_would():
         quantize_state_dict(stacked, fp8_modules=["v_proj"])
 
 
+def test_quantiser_refuses_an_expression_that_names_nothing(tmp_path):
+    from vllm_pq_amd.quantize import _main, quantize_state_dict
+    state = _attention_state()
+    for fp8, lost in ((["dwon_proj"], "dwon_proj"), (["down_proj", r"layers\.7\."], "layers"), (["norm"], "norm")):
+        with pytest.raises(ValueError, match=lost):
+            quantize_state_dict({**state, "model.norm.weight": torch.ones(128)}, iters=1, fp8_modules=fp8)
+    _checkpoint(tmp_path)
+    with pytest.raises(ValueError, match="o_proj"):
+        _main([str(tmp_path / "in"), str(tmp_path / "out"), "--iters", "1", "--device", "cpu", "--fp8", "o_proj"])
+    assert not (tmp_path / "out").exists()
+
+
 def test_method_raises_on_cpu():
     layer = ColumnParallelLinear(256, 128, bias=False, params_dtype=BF16, quant_config=PQConfig(fp8_modules=["."]), prefix="x")
     m, x = layer.quant_method, torch.zeros(2, 256, dtype=BF16)

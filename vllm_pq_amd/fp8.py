@@ -36,9 +36,9 @@ def is_fp8_module(prefix: str, patterns: List[str]) -> bool:
 def checkpoint_fp8_modules(modules: Iterable[str], patterns: List[str]) -> Set[str]:
     """Those of a checkpoint's modules that become e4m3 layers under `patterns`: a module goes by the layer that stacks it where
     the checkpoint holds all that this layer stacks, else by its own name, and either by is_fp8_module, as a model that loads
-    the checkpoint has it."""
+    the checkpoint has it.  An expression that names none of them is refused."""
     modules = set(modules)
-    found = set()
+    found, used = set(), set()
     for m in modules:
         head, _, last = m.rpartition(".")
         layer = m
@@ -47,6 +47,10 @@ def checkpoint_fp8_modules(modules: Iterable[str], patterns: List[str]) -> Set[s
                 layer = f"{head}.{fused}" if head else fused
         if is_fp8_module(layer, patterns):
             found.add(m)
+            used.update(p for p in patterns if re.search(p, m) or re.search(p, layer))
+    for p in patterns:
+        if p not in used:
+            raise ValueError(f"fp8_modules: {p!r} names none of the modules that are quantised")
     return found
 
 
