@@ -187,6 +187,15 @@ def test_quantiser_refuses_an_expression_that_names_nothing(tmp_path):
     assert not (tmp_path / "out").exists()
 
 
+def test_quantiser_refuses_stacked_matrices_of_odd_size():
+    from vllm_pq_amd.quantize import quantize_state_dict
+    state = {f"mlp.{n}.weight": _dense(i, 192, 128) for i, n in enumerate(("gate_proj", "up_proj"))}
+    with pytest.raises(ValueError, match="scale block"):
+        quantize_state_dict(state, fp8_modules=["gate_up_proj"])
+    alone = quantize_state_dict({"mlp.down_proj.weight": _dense(0, 192, 100)}, fp8_modules=["down_proj"])
+    assert alone["mlp.down_proj.weight_scale_inv"].shape == (2, 1)
+
+
 def test_method_raises_on_cpu():
     layer = ColumnParallelLinear(256, 128, bias=False, params_dtype=BF16, quant_config=PQConfig(fp8_modules=["."]), prefix="x")
     m, x = layer.quant_method, torch.zeros(2, 256, dtype=BF16)

@@ -10,7 +10,7 @@ Activations are quantised per token and group of 128 features when the layer run
 the step in front of the layer (apply_after_norm, apply_after_silu_and_mul).
 """
 import re
-from typing import Iterable, List, Optional, Set, Tuple
+from typing import Dict, List, Optional, Set, Tuple
 
 import torch
 from torch.nn.parameter import Parameter
@@ -33,19 +33,22 @@ def is_fp8_module(prefix: str, patterns: List[str]) -> bool:
     return bool(found) or any(re.search(p, prefix) for p in patterns)
 
 
-def checkpoint_fp8_modules(modules: Iterable[str], patterns: List[str]) -> Set[str]:
-    """Those of a checkpoint's modules that become e4m3 layers under `patterns`: a module goes by the layer that stacks it where
-    the checkpoint holds all that this layer stacks, else by its own name, and either by is_fp8_module, as a model that loads
-    the checkpoint has it.  An expression that names none of them is refused."""
-    modules = set(modules)
+def checkpoint_fp8_modules(modules: Dict[str, int], patterns: List[str]) -> Set[str]:
+    """Those of a checkpoint's modules (name: out_features) that become e4m3 layers under `patterns`: a module goes by the layer
+    that stacks it where the checkpoint holds all that this layer stacks, else by its own name, and either by is_fp8_module, as a
+    model that loads the checkpoint has it.  Refused: an expression that names none of them, and a stacked matrix whose rows do
+    not fill its scale blocks, which create_weights would not take."""
     found, used = set(), set()
-    for m in modules:
+    for m, rows in modules.items():
         head, _, last = m.rpartition(".")
         layer = m
         for fused, parts in _FUSED.items():
             if last in parts and all((f"{head}.{n}" if head else n) in modules for n in parts):
                 layer = f"{head}.{fused}" if head else fused
         if is_fp8_module(layer, patterns):
+            if layer != m and rows % ops.FP8_GROUP:
+                raise ValueError(f"{m}: {rows} output features are not a multiple of the scale block ({ops.FP8_GROUP}), which a part "
+                                 f"of {layer} has to be in e4m3")
             found.add(m)
             used.update(p for p in patterns if re.search(p, m) or re.search(p, layer))
     for p in patterns:

@@ -161,7 +161,7 @@ def quantize_state_dict(state: Dict[str, torch.Tensor], include: str = r".*(q_pr
     if isinstance(fp8_modules, str):
         raise ValueError(f"fp8_modules must be a list of regular expressions, got {fp8_modules!r}")
     pat = re.compile(include)
-    fp8 = checkpoint_fp8_modules([n[:-len(".weight")] for n, t in state.items() if t.dim() == 2 and pat.match(n)],
+    fp8 = checkpoint_fp8_modules({n[:-len(".weight")]: t.shape[0] for n, t in state.items() if t.dim() == 2 and pat.match(n)},
                                  fp8_modules) if fp8_modules else ()
     out: Dict[str, torch.Tensor] = {}
     for i, (name, t) in enumerate(state.items()):
