@@ -592,6 +592,23 @@ def test_gpu_offsets_past_32_bits(T, N, stride):
 
 
 @gpu
+@pytest.mark.parametrize("T,N,stride", [(1, 72, 2 ** 26 - 16), (1, 72, 2 ** 26), (5, 40, 2 ** 27)])
+def test_gpu_linear_of_few_tokens_and_rows_far_apart(T, N, stride):
+    """Tokens that are quantised inside the product's launch, and before it where the weight's rows are too far apart for that."""
+    K = 272
+    gen = torch.Generator().manual_seed(T + N)
+    x = activations(gen, T, K, torch.bfloat16).to(DEV)
+    w, ws = (t.to(DEV) for t in weight(gen, N, K))
+    bias = torch.randn(N, generator=gen).to(torch.bfloat16).to(DEV)
+    far = torch.empty(N * stride, dtype=torch.uint8, device=DEV).view(N, stride)[:, :K].copy_(w.view(torch.uint8)).view(F8)
+    q, s = ops.fp8_group_quant(x)
+    y = ops.fp8_block_linear(x, far, ws, bias)
+    check_gemm(y, q, s, w, ws, bias, DEV)
+    assert torch.equal(y, ops.fp8_block_linear(x, w, ws, bias))
+    assert torch.equal(y, ops.fp8_block_linear(x.view(1, T, K), far, ws, bias)[0])
+
+
+@gpu
 @pytest.mark.parametrize("T", [3, 16, 40, 300])
 @pytest.mark.parametrize("K", [256, 384, 1027, 4500])
 def test_gpu_a_token_stands_for_itself(T, K):

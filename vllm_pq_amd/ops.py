@@ -919,6 +919,9 @@ def _fp8_linear_impl(input: torch.Tensor, weight: torch.Tensor, weight_scales: t
         out = out.view(input.shape[:-1] + (N,))
     if T and N:
         nbytes = _fp8_tmp_bytes("pq_fp8_block_linear_tmp_bytes", T, N, K)
+        if w0 >> 26 and not nbytes and K:      # rows too far apart for the launch that quantises inside
+            q, s = _fp8_quant_impl("pq_fp8_group_quant", x2, 1)
+            return _fp8_gemm_impl(q, s, weight, weight_scales, bias, input.dtype).view(out.shape)
         tmp = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _call_on(dev, _lib.load().pq_fp8_block_linear, x2.data_ptr(), T, xs, weight.data_ptr(), w0, weight_scales.data_ptr(),
                  (K + FP8_GROUP - 1) // FP8_GROUP, bptr, N, K, code, out.data_ptr(), N, None if tmp is None else tmp.data_ptr(),
