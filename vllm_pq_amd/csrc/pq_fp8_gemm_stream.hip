@@ -25,7 +25,7 @@ namespace pq {
 constexpr int SM_WAVES = 8, SM_KPW = 4, SM_ROW = 20;   // waves; scale blocks of a wave at most; floats between tokens' sums
 constexpr int SM_RANGE = SM_WAVES * SM_KPW;            // scale blocks of a range of K
 constexpr size_t SM_SUM_BYTES = 2 * SM_WAVES * 16 * SM_ROW * sizeof(float);
-constexpr int SM_MAX_FUSED = 8192;                     // values a block quantises at most (8.5 KiB of LDS)
+constexpr int SM_MAX_FUSED = 8192;                     // values a block quantises at most (whole groups and scales: up to 9.7 KiB of LDS)
 
 typedef __attribute__((address_space(4))) float const_float;   // memory that no kernel running writes
 
