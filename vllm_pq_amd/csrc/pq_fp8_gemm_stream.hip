@@ -6,9 +6,9 @@
 // weights alone, the next tile's requested before the present ones are multiplied: the loads never drain.  A load shaped
 // like the matrix operand (lanes of a quad on four rows) runs at a quarter of a CU's rate, 38 GB/s measured, which is
 // still 1.5 times a CU's share of HBM.  The waves' sums meet in LDS once per tile, added in wave order.  A K of more than 32
-// scale blocks is cut into ranges (gridDim.y) whose sums are added by a second launch.  Bound by the weights' bytes: 16 tokens of
-// 28672 x 4096 27.8 us with weights from HBM (4.2 TB/s), 25.3 us where the last-level cache holds them; 1 token of 6144 x 4096
-// 9.2 us (2.7 TB/s, launch included).
+// scale blocks is cut into ranges (gridDim.y) whose sums are added by a second launch.  Bound by the weights' bytes: in a graph,
+// 16 tokens of 28672 x 4096 25.3 to 27.8 us with weights from HBM (4.2 to 4.6 TB/s), 22.0 where the last-level cache holds them; 1
+// token of 6144 x 4096 10.8 us (2.3 TB/s, launch included) and 8.7.
 //
 // FUSED takes fp16 / bf16 activations: the block quantises them itself into LDS while its first weights are on their way
 // (the same arithmetic as fp8_group_quant, so the same values), which saves a launch where there are few.

@@ -11,11 +11,12 @@
 // different groups of banks.  The DMA writes 64 lanes x 16 bytes in lane order, so it is the lanes' GLOBAL addresses that are
 // permuted; the 8 lanes of a row still read one 128-byte line.
 //
-// Measured: 4096 tokens of 28672 x 4096 411 to 440 us over several devices (2.2 to 2.35 PFLOP/s).  Of that the matrix
-// instructions alone take 268 us, with the LDS reads 296, with the sums 325; the rest is DMA and stores in the way of
-// both, at 1.9 GHz, which is what the power limit leaves of the clock.  512 tokens of 4096 x 4096 14.2 to 15.8 us (5 us of
-// it to start and end one round), 128 tokens of 4096 x 14336 18.4 us and 4 for adding the two ranges (a block has 48 KiB of
-// weights under way, and memory answers in 1.9 us).
+// Measured over several devices, in a graph: 4096 tokens of 28672 x 4096 404 to 440 us with the weights in the last-level cache
+// (2.2 to 2.4 PFLOP/s), 419 to 450 us from HBM; the first 20 calls after idleness 456 to 492.  Of 421 us the matrix
+// instructions alone take 268, with the LDS reads 296, with the sums 325; the rest is DMA and stores in the way of
+// both, at 1.9 GHz, which is what the power limit leaves of the clock.  512 tokens of 4096 x 4096 15.2 to 15.8 us (5 us of
+// it to start and end one round) and 18 from HBM; 128 tokens of 4096 x 14336 16.5 to 18.4 us and 4 for adding the two ranges, 27 in
+// all from HBM (a block has 48 KiB of weights under way, and memory answers in 1.9 us).
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <math.h>
