@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 // FAR is for gates beyond 88 on either side, of which there are none in most waves:
 //   - the exponential takes g as at most 128, where it is far below 1's last place, so that t stays finite at the type's
 //     largest value;
-//   - below -87.5 numerator and denominator carry 2^-125 more, which 2^t alone would not hold;
+//   - below -87.5 numerator and denominator carry a further 2^-125: 2^t itself leaves fp32 from -88.7 on;
 //   - below -174 g counts as 0: |silu(g) u| < 2^-115 for every finite u, less than half of the smallest value that e4m3 holds
 //     beside the floor's scale (2^-9 * 2^-96 / 448), so the type's lowest value gives nothing;
 //   - an infinity in g comes through u, as NaN.
